@@ -52,6 +52,7 @@ extern "C" {
 #define WLLM_TYPE_Q5_K 13
 #define WLLM_TYPE_Q6_K 14
 #define WLLM_TYPE_IQ4_XS 23
+#define WLLM_TYPE_BF16 30 /* activations and outputs of the 8-bit operators only */
 
 /* Descriptor geometry (matmul.ts:22-41): [op, n_src, dst block, src blocks...],
  * each block = buf_handle, offset, type, ne[4] lo, ne[4] hi, nb[4] lo, nb[4] hi.
@@ -292,6 +293,126 @@ int32_t wllm_mul_mat_prefill_static(int32_t src0_type, const void* w, int64_t w_
  * webllm_dequantize_q4_K (webgpu-bridge.cpp:692-708) on the device, for
  * Q4_K, Q5_K, Q6_K, Q4_0, Q8_0 and IQ4_XS. Returns -1 on bad arguments. */
 int32_t wllm_dequantize(int32_t type, const void* src, float* dst, int64_t n, void* stream);
+
+/* ---- 8-bit integer products and mixture-of-experts operators ----
+ * No counterpart in the reference. Beside MUL_MAT over GGUF blocks: products
+ * whose weights and activations are both int8, with a scale per channel (row of
+ * W) and per token, on the integer tensor cores; dense, or grouped by expert as
+ * ggml's MUL_MAT_ID groups them, with the router in front and the weighted sum
+ * behind.
+ *
+ * All of them take device pointers and a stream like wllm_mul_mat (NULL = the
+ * library stream; pass cudaStreamLegacy, (void*)1, for CUDA's default stream).
+ * They run on the device of wllm_init whatever the calling thread's current
+ * device is, use no library workspace, allocate nothing and never wait, so
+ * calls on several streams are independent and each may be captured into a
+ * graph. Inputs are not modified; an output may overlap no input of its call
+ * (WLLM_STATUS_FAILED where the library can see it). Extents are not checked.
+ * N = 0 tokens (rows) is allowed and does nothing. */
+
+/* N rows of K values to int8 with one scale each:
+ *   a = max_k |v_k|, scale = a / 127 in f32, q_k = the integer nearest v_k / scale
+ * (the exact quotient, ties to even, within -127..127; a = 0 gives q = 0). A row
+ * that holds a NaN or an infinity gets scale = NaN and q = 0, so its products
+ * are NaN. v is x, or
+ *   rms_norm != 0: x / sqrt(mean(x^2) + eps) * gain (gain: K floats or NULL);
+ *   glu != 0 (WLLM_GLU_*): act(x) * up, x the gate projection's output;
+ * not both. Rows are tokens' activations, or, once, a weight's channels (from
+ * wllm_dequantize, for example). Strides are in elements of x_type (F32, F16 or
+ * BF16; up has x's), q_stride in bytes. Bytes of q behind a row's K values are
+ * left as they are. */
+typedef struct wllm_quantize_i8_args {
+    int32_t x_type;
+    int32_t K, N;
+    int32_t glu;
+    const void* x;
+    int64_t x_stride;
+    const void* up;
+    int64_t up_stride;
+    const float* gain;
+    float eps;
+    int32_t rms_norm;
+    int8_t* q;
+    int64_t q_stride;
+    float* scale;
+} wllm_quantize_i8_args;
+int32_t wllm_quantize_i8(const wllm_quantize_i8_args* args, void* stream);
+
+/* y[m + y_stride*n] = (sum_k q[k + q_stride*n] * w[k + w_row_bytes*m])
+ *                     * q_scale[n] * w_scale[m]
+ * The sum is exact in int32 (K <= 131071); the scales are multiplied in f32 and
+ * the result rounded once to y_type (F32, F16 or BF16). Any M, N, K and strides;
+ * the tensor-core kernel takes w, q and their strides in multiples of 16 bytes
+ * (pad the rows: bytes behind K are not read), other addresses run on CUDA
+ * cores, much slower. */
+typedef struct wllm_mulmat_i8_args {
+    int32_t M, K, N;
+    int32_t y_type;
+    const int8_t* w;
+    int64_t w_row_bytes;
+    const float* w_scale; /* M */
+    const int8_t* q;
+    int64_t q_stride;     /* bytes */
+    const float* q_scale; /* N */
+    void* y;
+    int64_t y_stride;     /* elements of y_type */
+} wllm_mulmat_i8_args;
+int32_t wllm_mul_mat_i8(const wllm_mulmat_i8_args* args, void* stream);
+
+/* The router: of each token's n_expert logits (logits_type F32, F16 or BF16,
+ * logits_stride elements between tokens) the n_used largest, in falling order,
+ * equal ones by rising expert: ids[t*n_used + j] and weights[t*n_used + j].
+ * WLLM_MOE_SOFTMAX: exp(l) over the sum of all experts' exp, or, with
+ * normalize != 0, over the chosen ones'; WLLM_MOE_SIGMOID: 1 / (1 + exp(-l)),
+ * with normalize over the chosen ones' sum (0 if that is 0). Each times scale.
+ * A logit of NaN or -inf masks its expert: it is never chosen and no part of a
+ * sum; where fewer than n_used are left the rest get id -1 and weight 0. Logits
+ * of +inf share the softmax's weight evenly. n_expert <= 1024, n_used <= 32 and
+ * <= n_expert. */
+#define WLLM_MOE_SOFTMAX 0
+#define WLLM_MOE_SIGMOID 1
+int32_t wllm_moe_route(int32_t logits_type, const void* logits, int64_t logits_stride, int32_t n_tokens, int32_t n_expert,
+                       int32_t n_used, int32_t score, int32_t normalize, float scale, int32_t* ids, float* weights,
+                       void* stream);
+
+/* The slots s = t*n_used + j sorted by their expert ids[s], each expert's in
+ * rising order: expert e's are order[offsets[e]] .. order[offsets[e+1] - 1]
+ * (offsets: n_expert + 1 entries, order: n_tokens * n_used). Slots whose id is
+ * outside 0..n_expert-1 have no expert and come last, from
+ * order[offsets[n_expert]] on. The same expert may appear twice in a token. One
+ * plan serves every grouped product of a layer. */
+int32_t wllm_moe_plan(const int32_t* ids, int32_t n_tokens, int32_t n_used, int32_t n_expert, int32_t* offsets,
+                      int32_t* order, void* stream);
+
+/* MUL_MAT_ID in the form of wllm_mul_mat_i8, with W [n_expert][M][K]: slot s's
+ * row of y (y + y_stride*s) is its expert's product with row s of q
+ * (q_per_slot != 0) or row s / n_used (one row per token). offsets and order are
+ * wllm_moe_plan's for the same n_tokens, n_used and n_expert. Rows of slots
+ * without an expert are set to zero. */
+typedef struct wllm_mulmat_id_i8_args {
+    int32_t M, K;
+    int32_t n_expert, n_tokens, n_used;
+    int32_t q_per_slot;
+    int32_t y_type;
+    int32_t reserved; /* 0 */
+    const int8_t* w;
+    int64_t w_row_bytes, w_expert_bytes;
+    const float* w_scale; /* n_expert * M */
+    const int8_t* q;
+    int64_t q_stride;
+    const float* q_scale; /* n_tokens, or n_tokens * n_used */
+    const int32_t* offsets;
+    const int32_t* order;
+    void* y;
+    int64_t y_stride;
+} wllm_mulmat_id_i8_args;
+int32_t wllm_mul_mat_id_i8(const wllm_mulmat_id_i8_args* args, void* stream);
+
+/* y[m + y_stride*t] = sum_j weights[t*n_used + j] * z[m + z_stride*(t*n_used + j)],
+ * summed in f32 in the order of j and rounded once to y_type. z_type and y_type:
+ * F32, F16 or BF16. */
+int32_t wllm_moe_combine(int32_t z_type, const void* z, int64_t z_stride, const float* weights, int32_t y_type, void* y,
+                         int64_t y_stride, int32_t n_tokens, int32_t n_used, int32_t M, void* stream);
 
 /* Library build/version string. */
 const char* wllm_version(void);

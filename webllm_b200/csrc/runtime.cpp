@@ -708,11 +708,12 @@ int32_t wllm_sync(void) {
     e = cudaGetLastError();
     if (e != cudaSuccess) return cuda_fail(s, e, "wllm_sync (pending error)");
     const unsigned kerr = wllm::read_and_clear_stream_error() | (wllm::read_and_clear_prefill_error() << 8) |
-                          (wllm::read_and_clear_btc_error() << 16);
+                          (wllm::read_and_clear_btc_error() << 16) | (wllm::read_and_clear_i8_error() << 24);
     if (kerr)
         return fail(s,
                     "wllm_sync: a kernel gave up waiting (code 0x%x: bits 0-1 a pipeline barrier, 2 a row-sharded "
-                    "peer's signal, 3 an in-flight copy; bits 8-15 the prefill GEMM, 16+ the small-batch tcgen05 GEMM)",
+                    "peer's signal, 3 an in-flight copy; bits 8-15 the prefill GEMM, 16-23 the small-batch tcgen05 GEMM, 24+ the "
+                    "8-bit GEMM)",
                     kerr);
     return WLLM_STATUS_OK;
 }
@@ -1086,6 +1087,270 @@ int32_t wllm_graph_destroy(int32_t graph) {
     s.graphs.erase(it);
     s.graph_kernels.erase(graph);
     return WLLM_STATUS_OK;
+}
+
+// ---- 8-bit products and mixture-of-experts operators ----
+
+namespace {
+
+// (Arguments are checked ahead of the library's state, so a bad call is told
+// what is wrong with it on a host without a GPU too.)
+
+bool float_type(int32_t t) { return t == WLLM_TYPE_F32 || t == WLLM_TYPE_F16 || t == WLLM_TYPE_BF16; }
+int float_bytes(int32_t t) { return t == WLLM_TYPE_F32 ? 4 : 2; }
+
+// The library's device while a launch is made, then the caller's again.
+class OnDevice {
+public:
+    explicit OnDevice(const State& s) {
+        if (cudaGetDevice(&before_) != cudaSuccess) before_ = -1;
+        if (before_ != s.device) err_ = cudaSetDevice(s.device);
+        else before_ = -1;
+    }
+    ~OnDevice() {
+        if (before_ >= 0) cudaSetDevice(before_);
+    }
+    cudaError_t error() const { return err_; }
+
+private:
+    int before_ = -1;
+    cudaError_t err_ = cudaSuccess;
+};
+
+// Byte range of n rows of len elements, stride apart.
+ByteRange rows_range(const void* p, int64_t stride, int64_t n, int64_t len, int size) {
+    const uintptr_t b = reinterpret_cast<uintptr_t>(p);
+    return {b, b + (p && n > 0 ? static_cast<uintptr_t>(size) * static_cast<uintptr_t>(stride * (n - 1) + len) : 0)};
+}
+
+bool aligned(const void* p, int size) { return (reinterpret_cast<uintptr_t>(p) & (size - 1)) == 0; }
+
+// Counts a launch's kernels or reports its error.
+int32_t launched(State& s, const char* what, int rc) {
+    if (rc < 0) return cuda_fail(s, static_cast<cudaError_t>(-rc), what);
+    if (s.capturing) s.captured_kernels += static_cast<uint64_t>(rc);
+    else s.counters.kernels_launched += static_cast<uint64_t>(rc);
+    return WLLM_STATUS_OK;
+}
+
+constexpr int64_t kMaxStride = int64_t(1) << 39;  // what a tensor map's strides hold
+
+}  // namespace
+
+int32_t wllm_quantize_i8(const wllm_quantize_i8_args* a, void* stream) {
+    State& s = S();
+    std::lock_guard<std::mutex> g(s.mu);
+    const char* what = "wllm_quantize_i8";
+    if (!a) return fail(s, "%s: null args", what);
+    if (!float_type(a->x_type)) return fail(s, "%s: x_type %d is not F32, F16 or BF16", what, a->x_type);
+    if (a->K < 1 || a->N < 0) return fail(s, "%s: K=%d N=%d", what, a->K, a->N);
+    if (a->glu != 0 && a->glu != WLLM_GLU_SWIGLU && a->glu != WLLM_GLU_GELU)
+        return fail(s, "%s: unknown glu kind %d", what, a->glu);
+    if (a->glu && a->rms_norm) return fail(s, "%s: glu and rms_norm in one call", what);
+    if (a->rms_norm && !(a->eps >= 0.f && a->eps <= 1.f)) return fail(s, "%s: eps must be in [0, 1]", what);
+    if (a->N == 0) return ensure_init(s) ? WLLM_STATUS_OK : WLLM_STATUS_FAILED;
+    const int size = float_bytes(a->x_type);
+    if (!a->x || !a->q || !a->scale || (a->glu && !a->up)) return fail(s, "%s: null pointer", what);
+    if (!aligned(a->x, size) || (a->glu && !aligned(a->up, size)) || !aligned(a->scale, 4) || (a->rms_norm && !aligned(a->gain, 4)))
+        return fail(s, "%s: a pointer is not aligned to its type", what);
+    if (a->x_stride < 0 || a->up_stride < 0 || (a->N > 1 && a->q_stride < a->K))
+        return fail(s, "%s: x_stride=%lld up_stride=%lld q_stride=%lld (rows of q may not overlap)", what,
+                    (long long)a->x_stride, (long long)a->up_stride, (long long)a->q_stride);
+    const ByteRange q = rows_range(a->q, a->q_stride, a->N, a->K, 1), sc = rows_range(a->scale, 1, a->N, 1, 4);
+    const ByteRange in[3] = {rows_range(a->x, a->x_stride, a->N, a->K, size),
+                             rows_range(a->glu ? a->up : nullptr, a->up_stride, a->N, a->K, size),
+                             rows_range(a->rms_norm ? a->gain : nullptr, 0, 1, a->K, 4)};
+    for (const ByteRange& r : in)
+        if (overlap(q, r) || overlap(sc, r)) return fail(s, "%s: an output overlaps an input", what);
+    if (overlap(q, sc)) return fail(s, "%s: q overlaps scale", what);
+    wllm::QuantizeI8 o{};
+    o.x = a->x;
+    o.up = a->glu ? a->up : nullptr;
+    o.gain = a->rms_norm ? a->gain : nullptr;
+    o.q = a->q;
+    o.scale = a->scale;
+    o.x_stride = a->x_stride;
+    o.up_stride = a->up_stride;
+    o.q_stride = a->q_stride;
+    o.eps = a->eps;
+    o.x_type = a->x_type;
+    o.K = a->K;
+    o.N = a->N;
+    o.kind = a->rms_norm ? wllm::kProNorm
+                         : (a->glu == WLLM_GLU_SWIGLU ? wllm::kProSwiglu : (a->glu ? wllm::kProGelu : wllm::kProNone));
+    if (!ensure_init(s)) return WLLM_STATUS_FAILED;
+    const OnDevice dev(s);
+    if (dev.error() != cudaSuccess) return cuda_fail(s, dev.error(), what);
+    return launched(s, what, wllm::launch_quantize_i8(o, stream ? static_cast<cudaStream_t>(stream) : s.stream));
+}
+
+int32_t wllm_mul_mat_i8(const wllm_mulmat_i8_args* a, void* stream) {
+    State& s = S();
+    std::lock_guard<std::mutex> g(s.mu);
+    const char* what = "wllm_mul_mat_i8";
+    if (!a) return fail(s, "%s: null args", what);
+    if (!float_type(a->y_type)) return fail(s, "%s: y_type %d is not F32, F16 or BF16", what, a->y_type);
+    if (a->M < 1 || a->K < 1 || a->N < 0) return fail(s, "%s: M=%d K=%d N=%d", what, a->M, a->K, a->N);
+    if (a->K > wllm::kMaxK8) return fail(s, "%s: K=%d above %d (the int32 sum)", what, a->K, wllm::kMaxK8);
+    if (a->N == 0) return ensure_init(s) ? WLLM_STATUS_OK : WLLM_STATUS_FAILED;
+    const int size = float_bytes(a->y_type);
+    if (!a->w || !a->w_scale || !a->q || !a->q_scale || !a->y) return fail(s, "%s: null pointer", what);
+    if (!aligned(a->w_scale, 4) || !aligned(a->q_scale, 4) || !aligned(a->y, size))
+        return fail(s, "%s: a pointer is not aligned to its type", what);
+    if (a->w_row_bytes < a->K || a->q_stride < (a->N > 1 ? a->K : 0) || (a->N > 1 && a->y_stride < a->M) ||
+        a->w_row_bytes >= kMaxStride / a->M || a->q_stride >= kMaxStride || a->y_stride >= kMaxStride)
+        return fail(s, "%s: w_row_bytes=%lld q_stride=%lld (below K, or too large) or y_stride=%lld (below M)", what,
+                    (long long)a->w_row_bytes, (long long)a->q_stride, (long long)a->y_stride);
+    const ByteRange y = rows_range(a->y, a->y_stride, a->N, a->M, size);
+    if (overlap(y, rows_range(a->w, a->w_row_bytes, a->M, a->K, 1)) || overlap(y, rows_range(a->q, a->q_stride, a->N, a->K, 1)) ||
+        overlap(y, rows_range(a->w_scale, 1, a->M, 1, 4)) || overlap(y, rows_range(a->q_scale, 1, a->N, 1, 4)))
+        return fail(s, "%s: y overlaps an input", what);
+    wllm::MulMatI8 o{};
+    o.w = a->w;
+    o.q = a->q;
+    o.w_scale = a->w_scale;
+    o.q_scale = a->q_scale;
+    o.y = a->y;
+    o.w_row_bytes = a->w_row_bytes;
+    o.q_stride = a->N > 1 ? a->q_stride : (static_cast<int64_t>(a->K) + 15) / 16 * 16;
+    o.y_stride = a->y_stride;
+    o.M = a->M;
+    o.K = a->K;
+    o.N = a->N;
+    o.E = o.k = 1;
+    o.y_type = a->y_type;
+    if (!ensure_init(s)) return WLLM_STATUS_FAILED;
+    const OnDevice dev(s);
+    if (dev.error() != cudaSuccess) return cuda_fail(s, dev.error(), what);
+    return launched(s, what, wllm::launch_mul_mat_i8(o, stream ? static_cast<cudaStream_t>(stream) : s.stream, s.num_sms));
+}
+
+// n_tokens, n_used, n_expert as the mixture-of-experts entry points share them.
+static int32_t moe_sizes(State& s, const char* what, int32_t T, int32_t k, int32_t E) {
+    if (T < 0 || k < 1 || k > wllm::kMaxUsed || E < 1 || E > wllm::kMaxExperts)
+        return fail(s, "%s: n_tokens=%d n_used=%d (1..%d) n_expert=%d (1..%d)", what, T, k, wllm::kMaxUsed, E, wllm::kMaxExperts);
+    if (static_cast<int64_t>(T) * k > 0x7fffffffLL) return fail(s, "%s: n_tokens * n_used exceeds 2^31", what);
+    return WLLM_STATUS_OK;
+}
+
+int32_t wllm_moe_route(int32_t type, const void* logits, int64_t stride, int32_t T, int32_t E, int32_t k, int32_t score,
+                       int32_t normalize, float scale, int32_t* ids, float* weights, void* stream) {
+    State& s = S();
+    std::lock_guard<std::mutex> g(s.mu);
+    const char* what = "wllm_moe_route";
+    if (!float_type(type)) return fail(s, "%s: logits_type %d is not F32, F16 or BF16", what, type);
+    if (const int32_t rc = moe_sizes(s, what, T, k, E)) return rc;
+    if (k > E) return fail(s, "%s: n_used=%d of n_expert=%d", what, k, E);
+    if (score != WLLM_MOE_SOFTMAX && score != WLLM_MOE_SIGMOID) return fail(s, "%s: unknown score %d", what, score);
+    if (T == 0) return ensure_init(s) ? WLLM_STATUS_OK : WLLM_STATUS_FAILED;
+    const int size = float_bytes(type);
+    if (!logits || !ids || !weights) return fail(s, "%s: null pointer", what);
+    if (!aligned(logits, size) || !aligned(ids, 4) || !aligned(weights, 4))
+        return fail(s, "%s: a pointer is not aligned to its type", what);
+    if (stride < 0) return fail(s, "%s: negative stride", what);
+    const int64_t n = static_cast<int64_t>(T) * k;
+    const ByteRange in = rows_range(logits, stride, T, E, size), i = rows_range(ids, 1, n, 1, 4), w = rows_range(weights, 1, n, 1, 4);
+    if (overlap(in, i) || overlap(in, w) || overlap(i, w)) return fail(s, "%s: ids, weights and logits overlap", what);
+    const wllm::MoeRoute o{logits, stride, ids, weights, scale, type, T, E, k, score, normalize != 0};
+    if (!ensure_init(s)) return WLLM_STATUS_FAILED;
+    const OnDevice dev(s);
+    if (dev.error() != cudaSuccess) return cuda_fail(s, dev.error(), what);
+    return launched(s, what, wllm::launch_moe_route(o, stream ? static_cast<cudaStream_t>(stream) : s.stream));
+}
+
+int32_t wllm_moe_plan(const int32_t* ids, int32_t T, int32_t k, int32_t E, int32_t* offsets, int32_t* order, void* stream) {
+    State& s = S();
+    std::lock_guard<std::mutex> g(s.mu);
+    const char* what = "wllm_moe_plan";
+    if (const int32_t rc = moe_sizes(s, what, T, k, E)) return rc;
+    if (!offsets || (T > 0 && (!ids || !order))) return fail(s, "%s: null pointer", what);
+    if (!aligned(ids, 4) || !aligned(offsets, 4) || !aligned(order, 4)) return fail(s, "%s: a pointer is not aligned to its type", what);
+    const int64_t n = static_cast<int64_t>(T) * k;
+    const ByteRange i = rows_range(ids, 1, n, 1, 4), f = rows_range(offsets, 1, E + 1, 1, 4), r = rows_range(order, 1, n, 1, 4);
+    if (overlap(i, f) || overlap(i, r) || overlap(f, r)) return fail(s, "%s: ids, offsets and order overlap", what);
+    if (!ensure_init(s)) return WLLM_STATUS_FAILED;
+    const OnDevice dev(s);
+    if (dev.error() != cudaSuccess) return cuda_fail(s, dev.error(), what);
+    return launched(s, what, wllm::launch_moe_plan(ids, n, E, offsets, order, stream ? static_cast<cudaStream_t>(stream) : s.stream));
+}
+
+int32_t wllm_mul_mat_id_i8(const wllm_mulmat_id_i8_args* a, void* stream) {
+    State& s = S();
+    std::lock_guard<std::mutex> g(s.mu);
+    const char* what = "wllm_mul_mat_id_i8";
+    if (!a) return fail(s, "%s: null args", what);
+    if (!float_type(a->y_type)) return fail(s, "%s: y_type %d is not F32, F16 or BF16", what, a->y_type);
+    if (a->reserved != 0) return fail(s, "%s: reserved must be 0", what);
+    if (const int32_t rc = moe_sizes(s, what, a->n_tokens, a->n_used, a->n_expert)) return rc;
+    if (a->M < 1 || a->K < 1) return fail(s, "%s: M=%d K=%d", what, a->M, a->K);
+    if (a->K > wllm::kMaxK8) return fail(s, "%s: K=%d above %d (the int32 sum)", what, a->K, wllm::kMaxK8);
+    if (a->n_tokens == 0) return ensure_init(s) ? WLLM_STATUS_OK : WLLM_STATUS_FAILED;
+    const int size = float_bytes(a->y_type);
+    if (!a->w || !a->w_scale || !a->q || !a->q_scale || !a->offsets || !a->order || !a->y) return fail(s, "%s: null pointer", what);
+    if (!aligned(a->w_scale, 4) || !aligned(a->q_scale, 4) || !aligned(a->offsets, 4) || !aligned(a->order, 4) || !aligned(a->y, size))
+        return fail(s, "%s: a pointer is not aligned to its type", what);
+    const int64_t slots = static_cast<int64_t>(a->n_tokens) * a->n_used, rows = a->q_per_slot ? slots : a->n_tokens;
+    if (a->w_row_bytes < a->K || a->w_row_bytes >= kMaxStride / a->M ||
+        (a->n_expert > 1 && a->w_expert_bytes < a->w_row_bytes * (a->M - 1) + a->K) || a->w_expert_bytes >= kMaxStride ||
+        a->q_stride < (rows > 1 ? a->K : 0) || a->q_stride >= kMaxStride || (slots > 1 && a->y_stride < a->M) ||
+        a->y_stride >= kMaxStride)
+        return fail(s, "%s: w_row_bytes=%lld w_expert_bytes=%lld q_stride=%lld y_stride=%lld too small or too large for M=%d K=%d", what,
+                    (long long)a->w_row_bytes, (long long)a->w_expert_bytes, (long long)a->q_stride, (long long)a->y_stride, a->M, a->K);
+    const ByteRange y = rows_range(a->y, a->y_stride, slots, a->M, size);
+    const int64_t w_len = a->w_row_bytes * (a->M - 1) + a->K;
+    if (overlap(y, rows_range(a->w, a->w_expert_bytes, a->n_expert, w_len, 1)) || overlap(y, rows_range(a->q, a->q_stride, rows, a->K, 1)) ||
+        overlap(y, rows_range(a->w_scale, a->M, a->n_expert, a->M, 4)) || overlap(y, rows_range(a->q_scale, 1, rows, 1, 4)) ||
+        overlap(y, rows_range(a->offsets, 1, a->n_expert + 1, 1, 4)) || overlap(y, rows_range(a->order, 1, slots, 1, 4)))
+        return fail(s, "%s: y overlaps an input", what);
+    wllm::MulMatI8 o{};
+    o.w = a->w;
+    o.q = a->q;
+    o.w_scale = a->w_scale;
+    o.q_scale = a->q_scale;
+    o.y = a->y;
+    o.offsets = a->offsets;
+    o.order = a->order;
+    o.w_row_bytes = a->w_row_bytes;
+    o.w_expert_bytes = a->w_expert_bytes;
+    o.q_stride = rows > 1 ? a->q_stride : (static_cast<int64_t>(a->K) + 15) / 16 * 16;
+    o.y_stride = a->y_stride;
+    o.slots = slots;
+    o.M = a->M;
+    o.K = a->K;
+    o.N = static_cast<int32_t>(rows);
+    o.E = a->n_expert;
+    o.k = a->n_used;
+    o.per_slot = a->q_per_slot != 0;
+    o.y_type = a->y_type;
+    if (!ensure_init(s)) return WLLM_STATUS_FAILED;
+    const OnDevice dev(s);
+    if (dev.error() != cudaSuccess) return cuda_fail(s, dev.error(), what);
+    return launched(s, what, wllm::launch_mul_mat_id_i8(o, stream ? static_cast<cudaStream_t>(stream) : s.stream, s.num_sms));
+}
+
+int32_t wllm_moe_combine(int32_t z_type, const void* z, int64_t z_stride, const float* weights, int32_t y_type, void* y,
+                         int64_t y_stride, int32_t T, int32_t k, int32_t M, void* stream) {
+    State& s = S();
+    std::lock_guard<std::mutex> g(s.mu);
+    const char* what = "wllm_moe_combine";
+    if (!float_type(z_type) || !float_type(y_type)) return fail(s, "%s: types %d, %d are not F32, F16 or BF16", what, z_type, y_type);
+    if (const int32_t rc = moe_sizes(s, what, T, k, 1)) return rc;
+    if (M < 1) return fail(s, "%s: M=%d", what, M);
+    if (T == 0) return ensure_init(s) ? WLLM_STATUS_OK : WLLM_STATUS_FAILED;
+    if (!z || !weights || !y) return fail(s, "%s: null pointer", what);
+    const int zs = float_bytes(z_type), ys = float_bytes(y_type);
+    if (!aligned(z, zs) || !aligned(weights, 4) || !aligned(y, ys)) return fail(s, "%s: a pointer is not aligned to its type", what);
+    const int64_t slots = static_cast<int64_t>(T) * k;
+    if (z_stride < 0 || z_stride >= kMaxStride || (T > 1 && y_stride < M) || y_stride >= kMaxStride)
+        return fail(s, "%s: z_stride=%lld y_stride=%lld", what, (long long)z_stride, (long long)y_stride);
+    const ByteRange out = rows_range(y, y_stride, T, M, ys);
+    if (overlap(out, rows_range(z, z_stride, slots, M, zs)) || overlap(out, rows_range(weights, 1, slots, 1, 4)))
+        return fail(s, "%s: y overlaps an input", what);
+    const wllm::MoeCombine o{z, weights, y, z_stride, y_stride, z_type, y_type, T, k, M};
+    if (!ensure_init(s)) return WLLM_STATUS_FAILED;
+    const OnDevice dev(s);
+    if (dev.error() != cudaSuccess) return cuda_fail(s, dev.error(), what);
+    return launched(s, what, wllm::launch_moe_combine(o, stream ? static_cast<cudaStream_t>(stream) : s.stream));
 }
 
 const char* wllm_version(void) { return "wllm_mulmat 0.1 (sm_100a)"; }

@@ -9,12 +9,14 @@ namespace wllm {
 
 // GGUF block geometry (src/models/gguf-parser.ts:273-294).
 constexpr int kTypeF32 = 0;
+constexpr int kTypeF16 = 1;
 constexpr int kTypeQ4_0 = 2;
 constexpr int kTypeQ8_0 = 8;
 constexpr int kTypeQ4_K = 12;
 constexpr int kTypeQ5_K = 13;
 constexpr int kTypeQ6_K = 14;
 constexpr int kTypeIQ4_XS = 23;
+constexpr int kTypeBF16 = 30;
 
 inline int block_elems(int type) {
     switch (type) {
@@ -151,6 +153,73 @@ void* prefill_static_workspace(const char** err);
 
 // Workspace the launch of `ops` needs (0 if none).
 size_t mulmat_workspace_bytes(const MulMatOp* ops, int n_ops);
+
+// ---- 8-bit products and the mixture-of-experts operators ----
+// None of these uses library workspace: every buffer is the caller's, so calls
+// on several streams, and captured ones, share nothing. Each launcher returns
+// the number of kernels launched or a negative cudaError_t.
+
+// Rows to int8 with one scale each (i8_rows.cu).
+struct QuantizeI8 {
+    const void* x;
+    const void* up;     // kProSwiglu / kProGelu
+    const float* gain;  // kProNorm, or null
+    int8_t* q;
+    float* scale;
+    int64_t x_stride, up_stride;  // elements
+    int64_t q_stride;             // bytes
+    float eps;
+    int32_t x_type, K, N;
+    int32_t kind;  // ProKind
+};
+int launch_quantize_i8(const QuantizeI8& o, cudaStream_t stream);
+
+// y[row][m] = (sum_k q[..][k] w[e][m][k]) * q_scale * w_scale[e][m]
+// (mulmat_i8.cu): dense (E = 1, rows = N tokens), or grouped by expert (rows =
+// the `slots` entries of `order`, sorted by expert; offsets[e] where expert e's
+// begin). Grouped, slot s reads row s of q (per_slot) or row s / k.
+struct MulMatI8 {
+    const int8_t* w;
+    const int8_t* q;
+    const float* w_scale;
+    const float* q_scale;
+    void* y;
+    const int32_t* offsets;
+    const int32_t* order;
+    int64_t w_row_bytes, w_expert_bytes, q_stride;  // bytes
+    int64_t y_stride;                               // elements
+    int64_t slots;
+    int32_t M, K, N;  // N: rows of q
+    int32_t E, k;
+    int32_t per_slot, y_type;
+};
+constexpr int kMaxK8 = 131071;  // |sum| <= K * 128 * 128 < 2^31
+int launch_mul_mat_i8(const MulMatI8& o, cudaStream_t stream, int num_sms);
+int launch_mul_mat_id_i8(const MulMatI8& o, cudaStream_t stream, int num_sms);
+unsigned read_and_clear_i8_error();
+
+// Top-k router, slots by expert, weighted sum over a token's slots (moe.cu).
+constexpr int kMaxExperts = 1024;
+constexpr int kMaxUsed = 32;
+constexpr int kMoeSoftmax = 0, kMoeSigmoid = 1;
+struct MoeRoute {
+    const void* logits;
+    int64_t stride;  // elements
+    int32_t* ids;
+    float* weights;
+    float scale;
+    int32_t type, T, E, k, score, normalize;
+};
+int launch_moe_route(const MoeRoute& o, cudaStream_t stream);
+int launch_moe_plan(const int32_t* ids, int64_t slots, int E, int32_t* offsets, int32_t* order, cudaStream_t stream);
+struct MoeCombine {
+    const void* z;
+    const float* weights;
+    void* y;
+    int64_t z_stride, y_stride;  // elements
+    int32_t z_type, y_type, T, k, M;
+};
+int launch_moe_combine(const MoeCombine& o, cudaStream_t stream);
 
 // Device dequantization of n elements to f32 (bit-exact with the oracle).
 int launch_dequantize(int type, const void* src, float* dst, int64_t n, cudaStream_t stream);

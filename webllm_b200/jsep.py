@@ -38,6 +38,12 @@ GGML_TYPE_Q4_K = 12
 GGML_TYPE_Q5_K = 13
 GGML_TYPE_Q6_K = 14
 GGML_TYPE_IQ4_XS = 23
+GGML_TYPE_BF16 = 30  # activations and outputs of the 8-bit operators only
+
+MOE_SOFTMAX = 0  # exp(l) over a sum of exp (all experts, or the chosen ones)
+MOE_SIGMOID = 1  # 1 / (1 + exp(-l))
+
+STREAM_LEGACY = 1  # CUDA's default stream, for the stream arguments whose 0 is the library's
 
 TENSOR_BLOCK_I32 = 19
 
@@ -67,6 +73,7 @@ EXPORTED_SYMBOLS = (
     "wllm_graph_begin", "wllm_graph_end", "wllm_graph_launch", "wllm_graph_destroy",
     "wllm_dequantize", "wllm_version", "wllm_mul_mat_prefill_static",
     "wllm_ipc_alloc", "wllm_ipc_open", "wllm_ipc_close", "wllm_ipc_free", "wllm_mul_mat_batch_tp", "wllm_tp_wait", "wllm_set_wait_limit",
+    "wllm_quantize_i8", "wllm_mul_mat_i8", "wllm_moe_route", "wllm_moe_plan", "wllm_mul_mat_id_i8", "wllm_moe_combine",
 )
 
 MAX_RANKS = 8
@@ -90,6 +97,34 @@ class TpGroup(ctypes.Structure):
 class TpOutputs(ctypes.Structure):
     """wllm_tp_outputs (include/wllm_mulmat.h)."""
     _fields_ = [("y_rank", ctypes.c_void_p * MAX_RANKS)]
+
+
+class QuantizeI8Args(ctypes.Structure):
+    """wllm_quantize_i8_args (include/wllm_mulmat.h)."""
+    _fields_ = [("x_type", ctypes.c_int32), ("K", ctypes.c_int32), ("N", ctypes.c_int32), ("glu", ctypes.c_int32),
+                ("x", ctypes.c_void_p), ("x_stride", ctypes.c_int64), ("up", ctypes.c_void_p),
+                ("up_stride", ctypes.c_int64), ("gain", ctypes.c_void_p), ("eps", ctypes.c_float),
+                ("rms_norm", ctypes.c_int32), ("q", ctypes.c_void_p), ("q_stride", ctypes.c_int64),
+                ("scale", ctypes.c_void_p)]
+
+
+class MulMatI8Args(ctypes.Structure):
+    """wllm_mulmat_i8_args (include/wllm_mulmat.h)."""
+    _fields_ = [("M", ctypes.c_int32), ("K", ctypes.c_int32), ("N", ctypes.c_int32), ("y_type", ctypes.c_int32),
+                ("w", ctypes.c_void_p), ("w_row_bytes", ctypes.c_int64), ("w_scale", ctypes.c_void_p),
+                ("q", ctypes.c_void_p), ("q_stride", ctypes.c_int64), ("q_scale", ctypes.c_void_p),
+                ("y", ctypes.c_void_p), ("y_stride", ctypes.c_int64)]
+
+
+class MulMatIdI8Args(ctypes.Structure):
+    """wllm_mulmat_id_i8_args (include/wllm_mulmat.h)."""
+    _fields_ = [("M", ctypes.c_int32), ("K", ctypes.c_int32), ("n_expert", ctypes.c_int32),
+                ("n_tokens", ctypes.c_int32), ("n_used", ctypes.c_int32), ("q_per_slot", ctypes.c_int32),
+                ("y_type", ctypes.c_int32), ("reserved", ctypes.c_int32), ("w", ctypes.c_void_p),
+                ("w_row_bytes", ctypes.c_int64), ("w_expert_bytes", ctypes.c_int64), ("w_scale", ctypes.c_void_p),
+                ("q", ctypes.c_void_p), ("q_stride", ctypes.c_int64), ("q_scale", ctypes.c_void_p),
+                ("offsets", ctypes.c_void_p), ("order", ctypes.c_void_p), ("y", ctypes.c_void_p),
+                ("y_stride", ctypes.c_int64)]
 
 
 class WllmCounters(ctypes.Structure):
@@ -148,6 +183,12 @@ def load_library(path: str = LIB_PATH) -> ctypes.CDLL:
         "wllm_graph_launch": ([i32], i32),
         "wllm_graph_destroy": ([i32], i32),
         "wllm_version": ([], ctypes.c_char_p),
+        "wllm_quantize_i8": ([P(QuantizeI8Args), vp], i32),
+        "wllm_mul_mat_i8": ([P(MulMatI8Args), vp], i32),
+        "wllm_moe_route": ([i32, vp, i64, i32, i32, i32, i32, i32, ctypes.c_float, vp, vp, vp], i32),
+        "wllm_moe_plan": ([vp, i32, i32, i32, vp, vp, vp], i32),
+        "wllm_mul_mat_id_i8": ([P(MulMatIdI8Args), vp], i32),
+        "wllm_moe_combine": ([i32, vp, i64, vp, i32, vp, i64, i32, i32, i32, vp], i32),
     }
     for name, (argtypes, restype) in sig.items():
         fn = getattr(L, name)
@@ -545,3 +586,56 @@ def dequantize_device(qtype: int, src_ptr: int, dst_ptr: int, n: int, stream: in
     L = load_library()
     _check(L.wllm_dequantize(int(qtype), int(src_ptr), int(dst_ptr), int(n), int(stream) or None),
            "wllm_dequantize")
+
+
+# ---------------------------------------------------------------- 8-bit products, mixture of experts
+
+
+def quantize_i8(x_type: int, x_ptr: int, x_stride: int, N: int, K: int, q_ptr: int, q_stride: int, scale_ptr: int,
+                *, rms_norm: bool = False, gain_ptr: int = 0, eps: float = 0.0, glu: int = 0, up_ptr: int = 0,
+                up_stride: int = 0, stream: int = 0) -> int:
+    """N rows of K values to int8 with one scale each (wllm_quantize_i8): of x, of
+    RMS_NORM(x) * gain, or of act(x) * up. Strides: elements of x_type, q in bytes."""
+    a = QuantizeI8Args(x_type, K, N, glu, x_ptr, x_stride, up_ptr or None, up_stride, gain_ptr or None, eps,
+                       1 if rms_norm else 0, q_ptr, q_stride, scale_ptr)
+    return _check(load_library().wllm_quantize_i8(a, stream or None), "wllm_quantize_i8")
+
+
+def mul_mat_i8(w_ptr: int, w_row_bytes: int, w_scale_ptr: int, q_ptr: int, q_stride: int, q_scale_ptr: int,
+               y_type: int, y_ptr: int, y_stride: int, M: int, K: int, N: int, stream: int = 0) -> int:
+    """int8 product with a scale per channel and per token (wllm_mul_mat_i8)."""
+    a = MulMatI8Args(M, K, N, y_type, w_ptr, w_row_bytes, w_scale_ptr, q_ptr, q_stride, q_scale_ptr, y_ptr, y_stride)
+    return _check(load_library().wllm_mul_mat_i8(a, stream or None), "wllm_mul_mat_i8")
+
+
+def moe_route(logits_ptr: int, logits_stride: int, n_tokens: int, n_expert: int, n_used: int, score: int,
+              normalize: bool, scale: float, ids_ptr: int, weights_ptr: int, *, logits_type: int = GGML_TYPE_F32,
+              stream: int = 0) -> int:
+    """The n_used largest of each token's logits, and their weights (wllm_moe_route)."""
+    return _check(load_library().wllm_moe_route(logits_type, logits_ptr, logits_stride, n_tokens, n_expert, n_used,
+                                                score, 1 if normalize else 0, scale, ids_ptr, weights_ptr,
+                                                stream or None), "wllm_moe_route")
+
+
+def moe_plan(ids_ptr: int, n_tokens: int, n_used: int, n_expert: int, offsets_ptr: int, order_ptr: int,
+             stream: int = 0) -> int:
+    """The slots t*n_used + j sorted by expert (wllm_moe_plan)."""
+    return _check(load_library().wllm_moe_plan(ids_ptr, n_tokens, n_used, n_expert, offsets_ptr, order_ptr,
+                                               stream or None), "wllm_moe_plan")
+
+
+def mul_mat_id_i8(w_ptr: int, w_row_bytes: int, w_expert_bytes: int, w_scale_ptr: int, q_ptr: int, q_stride: int,
+                  q_scale_ptr: int, q_per_slot: bool, offsets_ptr: int, order_ptr: int, y_type: int, y_ptr: int,
+                  y_stride: int, M: int, K: int, n_expert: int, n_tokens: int, n_used: int, stream: int = 0) -> int:
+    """int8 products grouped by expert: a row of y per slot (wllm_mul_mat_id_i8)."""
+    a = MulMatIdI8Args(M, K, n_expert, n_tokens, n_used, 1 if q_per_slot else 0, y_type, 0, w_ptr, w_row_bytes,
+                       w_expert_bytes, w_scale_ptr, q_ptr, q_stride, q_scale_ptr, offsets_ptr, order_ptr, y_ptr,
+                       y_stride)
+    return _check(load_library().wllm_mul_mat_id_i8(a, stream or None), "wllm_mul_mat_id_i8")
+
+
+def moe_combine(z_type: int, z_ptr: int, z_stride: int, weights_ptr: int, y_type: int, y_ptr: int, y_stride: int,
+                n_tokens: int, n_used: int, M: int, stream: int = 0) -> int:
+    """Weighted sum over each token's slots (wllm_moe_combine)."""
+    return _check(load_library().wllm_moe_combine(z_type, z_ptr, z_stride, weights_ptr, y_type, y_ptr, y_stride,
+                                                  n_tokens, n_used, M, stream or None), "wllm_moe_combine")
