@@ -11,20 +11,31 @@
 // a single token and a prompt, a lane's column values are one channel's, and a
 // warp's store covers 32 consecutive channels of a token's row.
 //
-//  - warp 0 (TMA): per 128-byte chunk of K one box of 128 weight rows and the
-//    tile's token rows into a ring of stages (K-major, 128-byte swizzle). Dense
-//    tokens come as one box; an expert's tokens are gathered, four rows a copy
-//    (tile::gather4), through the sorted slots, so no sorted copy of the
-//    activations is ever written.
+//  - warp 0 (TMA): per 128-byte chunk of K one box of 128 weight rows, and of
+//    dense tokens one box of the tile's rows, into a ring of stages (K-major,
+//    128-byte swizzle).
+//  - warps 6..9 (grouped only): an expert's tokens are gathered through the
+//    sorted slots with 16-byte cp.async, straight into the swizzled layout, so
+//    no sorted copy of the activations is ever written. (TMA's gather of four
+//    rows a copy took 18 cycles a row: 1045 us against GATHER_US for 4096 tokens
+//    in 8 of 128 experts, 1536 -> 4096.)
 //  - warp 1 (MMA): one thread issues the 4 K=32 MMAs of a chunk.
 //  - warps 2..5 (epilogue): TMEM -> scales -> y, while the next tile's MMAs
-//    fill the other accumulator.
+//    fill the other accumulator. An item's rows and scales are fetched ahead of
+//    the wait for its accumulator.
 //
-// CTAs are persistent over the items (expert, channel tile, token tile). Where
-// the items are fewer than the SMs (single tokens, small batches), S = 2, 4 or
-// 8 CTAs of a cluster share an item's K: each leaves its int32 tile in its own
-// shared memory, and after a cluster barrier CTA r adds the S tiles of its
-// share of the columns through distributed shared memory.
+// CTAs are persistent over the items (expert, channel tile, token tile), in one
+// of three modes (plan() says which):
+//  - single: an item is 128 channels;
+//  - pair: two CTAs of a cluster share an item of 256 channels (cta_group::2):
+//    each loads its own 128 weight rows and half of the tokens, which both read,
+//    so a chunk of a 256-token tile takes 32 KB of an SM's L2 bandwidth instead
+//    of 48;
+//  - split: where the items are fewer than the SMs (single tokens, small
+//    batches), S = 2, 4 or 8 CTAs of a cluster share an item's K: each leaves
+//    its int32 tile in its own shared memory, and after a cluster barrier CTA r
+//    adds the S tiles of its share of the columns through distributed shared
+//    memory.
 //
 // Bounds: HBM (the weights, once) up to a few hundred tokens, the tensor pipe
 // above.
@@ -48,22 +59,34 @@ __device__ unsigned int g_i8_error = 0;
 namespace {
 
 constexpr int kTileM = 128;    // channels of a tile
-constexpr int kMaxTileN = 256; // tokens of a tile
-constexpr int kChunk = 128;    // bytes of K of a stage
+constexpr int kMaxTileN = 256; // tokens of a pair's tile
+constexpr int kMaxSingleN = 64; // of a single CTA's or a split one
+constexpr int kChunk = 128;    // bytes of K of a swizzled row
 constexpr int kABytes = kTileM * kChunk;
-constexpr int kThreads = 192;
+// Chunks of a stage. A stage costs its copy and MMA warps some 350 clocks of
+// waits and issue whatever its size; the 256-token MMAs of a pair's chunk take
+// 512, those of a single token far less, so there two chunks share a stage.
+template <int MODE>
+__host__ __device__ constexpr int chunks_of_stage();
+constexpr int kThreads = 192;       // copies, MMAs, four epilogue warps
+constexpr int kLoaders = 128;       // threads that gather tokens
 constexpr int kMaxStages = 12;
-constexpr int kSmemBytes = 220 * 1024;  // dynamic, beside about 5 KB of tables and barriers
+constexpr int kPrefetch = 16;       // chunks of weights brought into L2 ahead of the launch's dependency
+constexpr int kSmemBytes = 213 * 1024;  // dynamic, beside up to 13 KB of tables and barriers
 constexpr uint32_t kSpinLimit = 1u << 26;
 
 struct I8Args {
     CUtensorMap wmap;  // weights: [E][M][K] bytes, box 128 x 128 x 1
-    CUtensorMap xmap;  // tokens: [rows][K] bytes, box 128 x tile_n (dense) or 128 x 1 (gathered)
+    CUtensorMap xmap;  // dense tokens: [rows][K] bytes, box 128 x the tile's rows of one CTA
     MulMatI8 o;
-    int32_t tile_n;    // tokens of a full tile, a multiple of 16
-    int32_t tiles_m, chunks, stages, splits;
+    int32_t tile_n;    // tokens of a full tile, a multiple of 16 (pair: of 32)
+    int32_t tiles_m, chunks, stages, splits;  // chunks: of a stage's bytes of K
     int32_t tmem_cols;
 };
+
+enum Mode : int { kSingle = 0, kSplit = 1, kPair = 2 };
+template <int MODE>
+__host__ __device__ constexpr int chunks_of_stage() { return MODE == kPair ? 1 : 2; }
 
 __device__ __forceinline__ uint32_t smem_u32(const void* p) { return static_cast<uint32_t>(__cvta_generic_to_shared(p)); }
 __device__ __forceinline__ void mbar_init(uint64_t* bar, uint32_t count) {
@@ -114,14 +137,36 @@ __device__ __forceinline__ void tma_3d(uint32_t dst, const CUtensorMap* tm, int 
         "l"(tm), "r"(x), "r"(y), "r"(z), "r"(smem_u32(bar))
         : "memory");
 }
-// Four rows of 128 bytes from byte x on.
-__device__ __forceinline__ void tma_gather4(uint32_t dst, const CUtensorMap* tm, int x, int4 rows, uint64_t* bar) {
+// The same into this CTA's memory, signalled on the barrier of the pair's first CTA.
+__device__ __forceinline__ void tma_2d_pair(uint32_t dst, const CUtensorMap* tm, int x, int y, uint64_t* bar) {
     asm volatile(
-        "cp.async.bulk.tensor.2d.shared::cluster.global.tile::gather4.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5, "
-        "%6}], [%7];" ::"r"(dst),
-        "l"(tm), "r"(x), "r"(rows.x), "r"(rows.y), "r"(rows.z), "r"(rows.w), "r"(smem_u32(bar))
+        "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(
+            dst),
+        "l"(tm), "r"(x), "r"(y), "r"(smem_u32(bar) & 0xFEFFFFFFu)
         : "memory");
 }
+__device__ __forceinline__ void tma_3d_pair(uint32_t dst, const CUtensorMap* tm, int x, int y, int z, uint64_t* bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], "
+        "[%5];" ::"r"(dst),
+        "l"(tm), "r"(x), "r"(y), "r"(z), "r"(smem_u32(bar) & 0xFEFFFFFFu)
+        : "memory");
+}
+// 16 bytes to shared memory, zeros where bytes is 0.
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, uint32_t bytes) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+// Arrives on bar when this thread's cp.async so far have landed.
+__device__ __forceinline__ void cp_async_arrive(uint64_t* bar) {
+    asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
+// Arrives on the barrier at bar's place in CTA `rank` of the cluster.
+__device__ __forceinline__ void mbar_arrive_at(uint64_t* bar, uint32_t rank) {
+    uint32_t remote;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(smem_u32(bar)), "r"(rank));
+    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(remote) : "memory");
+}
+__device__ __forceinline__ void fence_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 __device__ __forceinline__ void tma_prefetch_3d(const CUtensorMap* tm, int x, int y, int z) {
     asm volatile("cp.async.bulk.prefetch.tensor.3d.L2.global.tile [%0, {%1, %2, %3}];" ::"l"(tm), "r"(x), "r"(y), "r"(z) : "memory");
 }
@@ -144,6 +189,22 @@ __device__ __forceinline__ void umma_i8(uint32_t tmem_d, uint64_t adesc, uint64_
         : "r"(tmem_d), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
         : "memory");
 }
+__device__ __forceinline__ void umma_i8_pair(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::i8 [%0], %1, %2, %3, p;\n\t}"
+        :
+        : "r"(tmem_d), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+// Arrives on bar in both CTAs of the pair when the MMAs so far are done.
+__device__ __forceinline__ void umma_commit_pair(uint64_t* bar) {
+    asm volatile(
+        "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(smem_u32(bar)),
+        "h"(static_cast<uint16_t>(3))
+        : "memory");
+}
 __device__ __forceinline__ void umma_commit(uint64_t* bar) {
     asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
 }
@@ -159,125 +220,195 @@ __device__ __forceinline__ void tmem_ld16(uint32_t taddr, int32_t (&r)[16]) {
         : "r"(taddr));
     asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 }
+// True in one lane of a converged warp. (Under `lane == 0` instead, the compiler
+// cannot tell that one thread issues a copy or an MMA, whose operands are
+// uniform registers, and wraps each in a loop over the active lanes: 700 clocks
+// a chunk where the MMAs take 512.)
+__device__ __forceinline__ bool elect_one() {
+    uint32_t p;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "elect.sync _|p, 0xffffffff;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(p));
+    return p != 0;
+}
+// A place in the ring of stages and the parity of its round.
+struct Ring {
+    int stages, s = 0;
+    uint32_t parity = 0;
+    __device__ __forceinline__ void next() {
+        if (++s == stages) s = 0, parity ^= 1;
+    }
+};
 __device__ __forceinline__ void cluster_sync() {
     asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
-__device__ __forceinline__ int32_t ld_cluster(uint32_t local, uint32_t rank) {
+__device__ __forceinline__ int4 ld_cluster4(uint32_t local, uint32_t rank) {
     uint32_t remote;
-    int32_t v;
+    int4 v;
     asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(local), "r"(rank));
-    asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(v) : "r"(remote) : "memory");
+    asm volatile("ld.shared::cluster.v4.s32 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+                 : "r"(remote)
+                 : "memory");
     return v;
 }
 
-// y[row][m] in y's type: the two scales in f32, then one rounding.
-__device__ __forceinline__ void store_y(const MulMatI8& o, int64_t row, int m, int32_t acc, float s, float t) {
-    const float v = __fmul_rn(__fmul_rn(__int2float_rn(acc), s), t);
+// y in its type: the two scales in f32, then one rounding.
+__device__ __forceinline__ float scaled(int32_t acc, float s, float t) { return __fmul_rn(__fmul_rn(__int2float_rn(acc), s), t); }
+__device__ __forceinline__ void put(float* p, float v) { *p = v; }
+__device__ __forceinline__ void put(__half* p, float v) { *p = __float2half_rn(v); }
+__device__ __forceinline__ void put(__nv_bfloat16* p, float v) { *p = __float2bfloat16_rn(v); }
+__device__ __forceinline__ void store_y(const MulMatI8& o, int64_t row, int m, float v) {
     const int64_t at = row * o.y_stride + m;
-    if (o.y_type == kTypeF32) static_cast<float*>(o.y)[at] = v;
-    else if (o.y_type == kTypeF16) static_cast<__half*>(o.y)[at] = __float2half_rn(v);
-    else static_cast<__nv_bfloat16*>(o.y)[at] = __float2bfloat16_rn(v);
-}
-__device__ __forceinline__ void zero_y(const MulMatI8& o, int64_t row, int m) {
-    const int64_t at = row * o.y_stride + m;
-    if (o.y_type == kTypeF32) static_cast<float*>(o.y)[at] = 0.f;
-    else static_cast<uint16_t*>(o.y)[at] = 0;
+    if (o.y_type == kTypeF32) put(static_cast<float*>(o.y) + at, v);
+    else if (o.y_type == kTypeF16) put(static_cast<__half*>(o.y) + at, v);
+    else put(static_cast<__nv_bfloat16*>(o.y) + at, v);
 }
 
 // An item: `rows` token rows from position `first` on, of expert e, against
-// channels m0.. . A group's token tiles are of one size (the least multiple of
-// 16 that covers it in as many tiles), its channel tiles come one after the
-// other with the token tiles of one channel tile next to each other (they read
-// the same weights).
+// the channels from m0 on. A group's token tiles are of one size (the least
+// multiple of 16, or 32 of a pair, that covers it in as many tiles), its channel
+// tiles come one after the other with the token tiles of one channel tile next
+// to each other (they read the same weights).
 struct Item {
     int e, m0, first, rows;
 };
 
-// Rows of each of the `tiles` tiles of a group of n.
-__device__ __forceinline__ int tile_rows(int n, int tiles) { return ((n + tiles - 1) / tiles + 15) & ~15; }
+// Walks the items i of a CTA in rising order. cum[e]: token tiles of the experts
+// before e, begin[e]: their slots (grouped; E + 1 entries each).
+template <bool GROUPED, int MODE>
+struct Walk {
+    const I8Args& P;
+    const int32_t* cum;
+    const int32_t* begin;
+    int e = 0;
 
-// cum[e]: token tiles of the experts before e (GROUPED); E + 1 entries.
-template <bool GROUPED>
-__device__ __forceinline__ Item item_of(const I8Args& P, const int32_t* cum, int64_t i) {
-    Item it;
-    if constexpr (!GROUPED) {
-        const int tiles = (P.o.N + P.tile_n - 1) / P.tile_n;
-        it.e = 0;
-        it.m0 = static_cast<int>(i / tiles) * kTileM;
-        it.first = static_cast<int>(i % tiles) * P.tile_n;
-        it.rows = min(P.tile_n, P.o.N - it.first);
-    } else {
-        const int64_t u = i / P.tiles_m;  // the token tile that holds the item if groups had one channel tile
-        int lo = 0, hi = P.o.E - 1;       // the last expert whose first tile is at or before u
-        while (lo < hi) {
-            const int mid = (lo + hi + 1) >> 1;
-            if (cum[mid] <= u) lo = mid;
-            else hi = mid - 1;
+    __device__ __forceinline__ Item at(int i) {
+        constexpr int kM = MODE == kPair ? 2 * kTileM : kTileM;
+        constexpr int kStep = MODE == kPair ? 32 : 16;
+        Item it;
+        if constexpr (!GROUPED) {
+            const int tiles = (P.o.N + P.tile_n - 1) / P.tile_n;
+            it.e = 0;
+            it.m0 = i / tiles * kM;
+            it.first = i % tiles * P.tile_n;
+            it.rows = min(P.tile_n, P.o.N - it.first);
+        } else {
+            while (cum[e + 1] * P.tiles_m <= i) ++e;
+            const int tiles = cum[e + 1] - cum[e], j = i - cum[e] * P.tiles_m;
+            const int n = begin[e + 1] - begin[e], size = ((n + tiles - 1) / tiles + kStep - 1) / kStep * kStep;
+            it.e = e;
+            it.m0 = j / tiles * kM;
+            it.first = begin[e] + j % tiles * size;
+            it.rows = min(size, begin[e + 1] - it.first);
         }
-        const int tiles = cum[lo + 1] - cum[lo];
-        const int j = static_cast<int>(i - static_cast<int64_t>(cum[lo]) * P.tiles_m);
-        const int begin = P.o.offsets[lo], n = P.o.offsets[lo + 1] - begin;
-        const int size = tile_rows(n, tiles);
-        it.e = lo;
-        it.m0 = (j / tiles) * kTileM;
-        it.first = begin + (j % tiles) * size;
-        it.rows = min(size, begin + n - it.first);
+        return it;
     }
-    return it;
+};
+
+// The rows of an accumulator that this warp holds, into y: column n of the tile
+// is token row[n] with scale s[n].
+template <typename T>
+__device__ __forceinline__ void store_tile(const MulMatI8& o, uint32_t taddr, int rows, int m, float tm, const int32_t* row,
+                                           const float* s) {
+    T* y = static_cast<T*>(o.y) + m;
+    const bool live = m < o.M;
+    int n = 0;
+    if (__all_sync(0xffffffffu, live)) {  // no branch between the 16 stores
+        for (; n + 16 <= rows; n += 16) {
+            int32_t acc[16];
+            tmem_ld16(taddr + n, acc);
+#pragma unroll
+            for (int j = 0; j < 16; ++j) put(y + row[n + j] * o.y_stride, scaled(acc[j], s[n + j], tm));
+        }
+    }
+    for (; n < rows; n += 16) {
+        int32_t acc[16];
+        tmem_ld16(taddr + n, acc);
+#pragma unroll
+        for (int j = 0; j < 16; ++j)
+            if (n + j < rows && live) put(y + row[n + j] * o.y_stride, scaled(acc[j], s[n + j], tm));
+    }
 }
 
-// GROUPED: tokens by expert. SPLIT: a cluster of P.splits CTAs shares an item's
-// K (one item per cluster).
-template <bool GROUPED, bool SPLIT>
-__global__ void __launch_bounds__(kThreads, 1) i8_kernel(const __grid_constant__ I8Args P) {
+template <bool GROUPED, int MODE>
+__global__ void __launch_bounds__(GROUPED ? kThreads + kLoaders : kThreads, 1) i8_kernel(const __grid_constant__ I8Args P) {
+    constexpr bool SPLIT = MODE == kSplit, PAIR = MODE == kPair;
     extern __shared__ __align__(1024) uint8_t smem_raw[];
-    __shared__ uint64_t full[kMaxStages], empty[kMaxStages], acc_full[2], acc_free[2];
+    __shared__ uint64_t full[kMaxStages], b_full[kMaxStages], empty[kMaxStages], acc_full[2], acc_free[2];
     __shared__ uint32_t tmem_slot;
     __shared__ int poison;
-    __shared__ int32_t cum[GROUPED ? kMaxExperts + 1 : 1];
-    __shared__ int32_t warp_sum[GROUPED ? kThreads / 32 : 1];
+    __shared__ int32_t cum[GROUPED ? kMaxExperts + 1 : 1], begin[GROUPED ? kMaxExperts + 1 : 1];
+    __shared__ int32_t warp_sum[10];
+    __shared__ int32_t out_row[2][PAIR ? kMaxTileN : kMaxSingleN];
+    __shared__ float out_scale[2][PAIR ? kMaxTileN : kMaxSingleN];
     // 1024-byte alignment for the swizzled tiles
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     volatile int* poisoned = &poison;
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int stages = P.stages, stage_bytes = kABytes + P.tile_n * kChunk;
-    const uint32_t rank = SPLIT ? blockIdx.x % P.splits : 0;
+    constexpr int kSub = chunks_of_stage<MODE>();
+    const int stages = P.stages, b_bytes = (PAIR ? P.tile_n / 2 : P.tile_n) * kChunk;
+    const int stage_bytes = kSub * (kABytes + b_bytes);  // kSub weight chunks, then as many of the tokens
+    uint32_t rank = 0;  // in the cluster
+    if constexpr (MODE != kSingle) asm volatile("mov.u32 %0, %cluster_ctarank;" : "=r"(rank));
     const int c0 = SPLIT ? static_cast<int>(static_cast<int64_t>(P.chunks) * rank / P.splits) : 0;
     const int c1 = SPLIT ? static_cast<int>(static_cast<int64_t>(P.chunks) * (rank + 1) / P.splits) : P.chunks;
-    const int64_t item0 = SPLIT ? blockIdx.x / P.splits : blockIdx.x;
-    const int64_t item_step = SPLIT ? gridDim.x / P.splits : gridDim.x;
+    const int group = SPLIT ? P.splits : (PAIR ? 2 : 1);  // CTAs that share an item
+    const int item0 = blockIdx.x / group, item_step = gridDim.x / group;
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < stages; ++s) {
-            mbar_init(&full[s], 1);
+            mbar_init(&full[s], PAIR && GROUPED ? 2 : 1);
+            mbar_init(&b_full[s], kLoaders);
             mbar_init(&empty[s], 1);
         }
         for (int b = 0; b < 2; ++b) {
             mbar_init(&acc_full[b], 1);
-            mbar_init(&acc_free[b], 4);
+            mbar_init(&acc_free[b], PAIR ? 8 : 4);
         }
         poison = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         asm volatile("prefetch.tensormap [%0];" ::"l"(&P.wmap) : "memory");
-        asm volatile("prefetch.tensormap [%0];" ::"l"(&P.xmap) : "memory");
+        if constexpr (!GROUPED) asm volatile("prefetch.tensormap [%0];" ::"l"(&P.xmap) : "memory");
     }
     if (warp == 1) {
-        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_slot)),
-                     "r"(P.tmem_cols));
-        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+        if constexpr (PAIR) {
+            asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_slot)),
+                         "r"(P.tmem_cols));
+            asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;");
+        } else {
+            asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_slot)),
+                         "r"(P.tmem_cols));
+            asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+        }
     }
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    if constexpr (!GROUPED) {
+        // The kernel before this one (the quantiser, as a rule) may still run: its
+        // writes are not read here, but the first item's weights can come into L2
+        // meanwhile (L2 is coherent, so this is safe even if they are being written).
+        if (threadIdx.x == 0 && item0 < (P.o.N + P.tile_n - 1) / P.tile_n * P.tiles_m) {
+            const int m0 = Walk<GROUPED, MODE>{P, nullptr, nullptr}.at(item0).m0 + (PAIR ? kTileM * rank : 0);
+            for (int c = kSub * c0; c < kSub * c1 && c < kSub * c0 + kPrefetch; ++c) tma_prefetch_3d(&P.wmap, c * kChunk, m0, 0);
+        }
+    }
     asm volatile("griddepcontrol.wait;" ::: "memory");
 
-    int64_t items;
+    int items;
     if constexpr (GROUPED) {
         // token tiles of each expert, then their running sum
         int carry = 0;
-        for (int base = 0; base < P.o.E; base += kThreads) {
+        for (int base = 0; base < P.o.E; base += blockDim.x) {
             const int e = base + threadIdx.x;
             int tiles = 0;
-            if (e < P.o.E) tiles = (P.o.offsets[e + 1] - P.o.offsets[e] + P.tile_n - 1) / P.tile_n;
+            if (e < P.o.E) {
+                const int at = P.o.offsets[e];
+                begin[e] = at;
+                tiles = (P.o.offsets[e + 1] - at + P.tile_n - 1) / P.tile_n;
+            }
             int sum = tiles;
 #pragma unroll
             for (int o = 1; o < 32; o <<= 1) {
@@ -288,176 +419,272 @@ __global__ void __launch_bounds__(kThreads, 1) i8_kernel(const __grid_constant__
             if (lane == 31) warp_sum[warp] = sum;
             __syncthreads();
             int before = carry;
-            for (int w = 0; w < kThreads / 32; ++w) {
+            for (int w = 0; w < (kThreads + kLoaders) / 32; ++w) {
                 if (w < warp) before += warp_sum[w];
                 carry += warp_sum[w];
             }
             if (e < P.o.E) cum[e + 1] = before + sum;
         }
-        if (threadIdx.x == 0) cum[0] = 0;
-        items = static_cast<int64_t>(carry) * P.tiles_m;
+        if (threadIdx.x == 0) {
+            cum[0] = 0;
+            begin[P.o.E] = P.o.offsets[P.o.E];
+        }
+        items = carry * P.tiles_m;
     } else {
-        items = static_cast<int64_t>((P.o.N + P.tile_n - 1) / P.tile_n) * P.tiles_m;
+        items = (P.o.N + P.tile_n - 1) / P.tile_n * P.tiles_m;
     }
     tc_fence_before();
-    __syncthreads();
+    if constexpr (PAIR) cluster_sync();  // the other CTA's barriers are set up too
+    else __syncthreads();
     tc_fence_after();
     const uint32_t tmem = tmem_slot;
+    Walk<GROUPED, MODE> walk{P, cum, begin};
 
     if (warp == 0) {
         // ---------------- copies ----------------
-        uint32_t q = 0;  // stages filled so far
+        Ring ring{stages};
+        int filled = 0;  // stages filled so far, up to the ring's size
         bool ok = true;
-        for (int64_t i = item0; i < items && ok; i += item_step) {
-            const Item it = item_of<GROUPED>(P, cum, i);
-            const int cols = (it.rows + 15) & ~15;
-            int4 rows[2];
-            if constexpr (GROUPED) {
-                // copies lane and lane + 32 of the item: four token rows each; what
-                // is behind the last row reads that row again
-#pragma unroll
-                for (int g = 0; g < 2; ++g) {
-                    int r[4];
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        const int slot = P.o.order[it.first + min((lane + 32 * g) * 4 + j, it.rows - 1)];
-                        r[j] = P.o.per_slot ? slot : slot / P.o.k;
+        for (int i = item0; i < items && ok; i += item_step) {
+            const Item it = walk.at(i);
+            const int m0 = it.m0 + (PAIR ? kTileM * rank : 0);
+            const int cols = (it.rows + 31) & ~31, n0 = it.first + (PAIR ? rank * (cols / 2) : 0);
+            for (int c = c0; c < c1; ++c) {
+                const int s = ring.s;
+                ok = filled < stages || mbar_wait(&empty[s], ring.parity ^ 1, 1u, poisoned);
+                ok = __all_sync(0xffffffffu, ok);
+                if (!ok) break;
+                const uint32_t a = smem_u32(smem + s * stage_bytes);
+                if (elect_one()) {
+                    const uint32_t b = a + kSub * kABytes;
+                    if constexpr (PAIR) {
+                        if (rank == 0) mbar_expect_tx(&full[s], 2 * (GROUPED ? kSub * kABytes : stage_bytes));
+                    } else {
+                        mbar_expect_tx(&full[s], GROUPED ? kSub * kABytes : stage_bytes);
                     }
-                    rows[g] = make_int4(r[0], r[1], r[2], r[3]);
+#pragma unroll
+                    for (int h = 0; h < kSub; ++h) {
+                        const int k = (c * kSub + h) * kChunk;
+                        if constexpr (PAIR) {
+                            tma_3d_pair(a + h * kABytes, &P.wmap, k, m0, it.e, &full[s]);
+                            if constexpr (!GROUPED) tma_2d_pair(b + h * b_bytes, &P.xmap, k, n0, &full[s]);
+                        } else {
+                            tma_3d(a + h * kABytes, &P.wmap, k, m0, it.e, &full[s]);
+                            if constexpr (!GROUPED) tma_2d(b + h * b_bytes, &P.xmap, k, n0, &full[s]);
+                        }
+                    }
                 }
+                __syncwarp();
+                if (filled < stages) ++filled;
+                ring.next();
             }
-            for (int c = c0; c < c1; ++c, ++q) {
-                const int s = q % stages;
-                if (q >= static_cast<uint32_t>(stages) && !mbar_wait(&empty[s], ((q / stages) - 1) & 1, 1u, poisoned)) {
-                    ok = false;
-                    break;
-                }
-                const uint32_t a = smem_u32(smem + s * stage_bytes), b = a + kABytes;
-                if constexpr (GROUPED) {
-                    if (lane == 0) {
-                        mbar_expect_tx(&full[s], kABytes + cols * kChunk);
-                        tma_3d(a, &P.wmap, c * kChunk, it.m0, it.e, &full[s]);
+        }
+        if (*poisoned && rank == 0) {  // the copies in flight land before the CTA ends
+            for (int p = 0; p < filled; ++p) {
+                ring.s = ring.s ? ring.s - 1 : (ring.parity ^= 1, stages - 1);
+                mbar_drain(&full[ring.s], ring.parity);
+            }
+        }
+    } else if (warp == 1) {
+        Ring ring{stages};
+        bool ok = true;
+        if (!PAIR || rank == 0) {
+            // ---------------- MMAs ----------------
+            uint32_t t = 0;
+            uint64_t* last = nullptr;  // the barrier of the last commit, and its parity
+            uint32_t last_parity = 0;
+            for (int i = item0; i < items && ok; i += item_step, ++t) {
+                const Item it = walk.at(i);
+                const uint32_t idesc = PAIR ? i8_idesc(2 * kTileM, (it.rows + 31) & ~31) : i8_idesc(kTileM, (it.rows + 15) & ~15);
+                const uint32_t buf = t & 1, d = tmem + buf * P.tile_n;
+                ok = t < 2 || mbar_wait(&acc_free[buf], ((t >> 1) - 1) & 1, 2u, poisoned);
+                ok = __all_sync(0xffffffffu, ok);
+                if (!ok) break;
+                tc_fence_after();
+                for (int c = c0; c < c1; ++c) {
+                    const int s = ring.s;
+                    ok = mbar_wait(&full[s], ring.parity, 4u, poisoned);
+                    if constexpr (GROUPED) {
+                        ok = ok && mbar_wait(&b_full[s], ring.parity, 4u, poisoned);
+                        fence_async();  // the gathered tokens were written by the generic proxy
+                    }
+                    ok = __all_sync(0xffffffffu, ok);
+                    if (!ok) break;
+                    tc_fence_after();
+                    const uint32_t a = smem_u32(smem + s * stage_bytes);
+                    if (elect_one()) {
+#pragma unroll
+                        for (int h = 0; h < kSub; ++h) {
+                            const uint64_t ad = umma_desc(a + h * kABytes), bd = umma_desc(a + kSub * kABytes + h * b_bytes);
+#pragma unroll
+                            for (int j = 0; j < kChunk / 32; ++j) {
+                                const uint32_t more = c > c0 || h > 0 || j > 0;
+                                if constexpr (PAIR) umma_i8_pair(d, ad + 2 * j, bd + 2 * j, idesc, more);
+                                else umma_i8(d, ad + 2 * j, bd + 2 * j, idesc, more);
+                            }
+                        }
+                        if constexpr (PAIR) umma_commit_pair(&empty[s]);
+                        else umma_commit(&empty[s]);
                     }
                     __syncwarp();
-                    for (int g = 0; g < 2; ++g)
-                        if ((lane + 32 * g) * 4 < cols)
-                            tma_gather4(b + (lane + 32 * g) * 4 * kChunk, &P.xmap, c * kChunk, g ? rows[1] : rows[0], &full[s]);
-                } else if (lane == 0) {
-                    mbar_expect_tx(&full[s], kABytes + P.tile_n * kChunk);
-                    tma_3d(a, &P.wmap, c * kChunk, it.m0, 0, &full[s]);
-                    tma_2d(b, &P.xmap, c * kChunk, it.first, &full[s]);
+                    last = &empty[s], last_parity = ring.parity;
+                    ring.next();
+                }
+                if (elect_one()) {
+                    if constexpr (PAIR) umma_commit_pair(&acc_full[buf]);
+                    else umma_commit(&acc_full[buf]);
                 }
                 __syncwarp();
             }
-            ok = __all_sync(0xffffffffu, ok);
-        }
-        if (!ok || *poisoned) {  // the copies in flight land before the CTA ends
-            for (uint32_t p = q > static_cast<uint32_t>(stages) ? q - stages : 0; p < q; ++p)
-                mbar_drain(&full[p % stages], (p / stages) & 1);
-        }
-    } else if (warp == 1) {
-        // ---------------- MMAs ----------------
-        if (lane == 0) {
-            uint32_t q = 0, t = 0;
-            bool ok = true;
-            for (int64_t i = item0; i < items && ok; i += item_step, ++t) {
-                const Item it = item_of<GROUPED>(P, cum, i);
-                const uint32_t idesc = i8_idesc(kTileM, (it.rows + 15) & ~15);
-                const uint32_t buf = t & 1, d = tmem + buf * P.tile_n;
-                if (t >= 2 && !mbar_wait(&acc_free[buf], ((t >> 1) - 1) & 1, 2u, poisoned)) break;
-                tc_fence_after();
-                for (int c = c0; c < c1; ++c, ++q) {
-                    const int s = q % stages;
-                    if (!mbar_wait(&full[s], (q / stages) & 1, 4u, poisoned)) {
-                        ok = false;
-                        break;
-                    }
-                    tc_fence_after();
-                    const uint32_t a = smem_u32(smem + s * stage_bytes);
-                    const uint64_t ad = umma_desc(a), bd = umma_desc(a + kABytes);
-#pragma unroll
-                    for (int j = 0; j < kChunk / 32; ++j) umma_i8(d, ad + 2 * j, bd + 2 * j, idesc, c > c0 || j > 0);
-                    umma_commit(&empty[s]);
-                }
-                umma_commit(&acc_full[buf]);
-            }
             // MMAs still in flight (only after a time-out) end before the TMEM is freed
-            if (*poisoned && q > 0) mbar_drain(&empty[(q - 1) % stages], ((q - 1) / stages) & 1);
+            if (*poisoned && last) mbar_drain(last, last_parity);
+        } else if constexpr (GROUPED) {
+            // ---------------- this CTA's tokens are ready, told to the pair's first ----------------
+            for (int i = item0; i < items && ok; i += item_step)
+                for (int c = c0; c < c1; ++c) {
+                    ok = mbar_wait(&b_full[ring.s], ring.parity, 4u, poisoned);
+                    if (!ok) break;
+                    fence_async();
+                    if (lane == 0) mbar_arrive_at(&full[ring.s], 0);
+                    ring.next();
+                }
         }
-    } else {
+    } else if (warp < 6) {
         // ---------------- epilogue ----------------
         const int quad = warp & 3;  // the TMEM lanes this warp may read
         uint32_t t = 0;
-        for (int64_t i = item0; i < items; i += item_step, ++t) {
-            const Item it = item_of<GROUPED>(P, cum, i);
+        for (int i = item0; i < items; i += item_step, ++t) {
+            const Item it = walk.at(i);
             const uint32_t buf = t & 1;
-            const int m = it.m0 + 32 * quad + lane;
+            const int m = it.m0 + (PAIR ? kTileM * rank : 0) + 32 * quad + lane;
             const float tm = m < P.o.M ? P.o.w_scale[static_cast<int64_t>(it.e) * P.o.M + m] : 0.f;
-            if (!mbar_wait(&acc_full[buf], (t >> 1) & 1, 2u, poisoned)) break;
+            for (int n = threadIdx.x - 64; n < it.rows; n += 128) {
+                int row = it.first + n;
+                if constexpr (GROUPED) row = P.o.order[row];
+                out_row[buf][n] = row;
+                out_scale[buf][n] = P.o.q_scale[!GROUPED || P.o.per_slot ? row : row / P.o.k];
+            }
+            asm volatile("bar.sync 1, 128;" ::: "memory");  // the epilogue warps
+            // after a time-out the items are still walked (the four warps meet at the
+            // barrier above), without their stores
+            const bool ok = mbar_wait(&acc_full[buf], (t >> 1) & 1, 2u, poisoned);
             tc_fence_after();
-            for (int n = 0; n < it.rows; n += 16) {
-                int32_t acc[16];
-                tmem_ld16(tmem + buf * P.tile_n + n + (static_cast<uint32_t>(32 * quad) << 16), acc);
-                if constexpr (SPLIT) {
-                    // the stages are free by now: all copies have landed and all MMAs have read them
-                    int32_t* part = reinterpret_cast<int32_t*>(smem);
+            const uint32_t d = tmem + buf * P.tile_n + (static_cast<uint32_t>(32 * quad) << 16);
+            if (!ok) {
+            } else if constexpr (SPLIT) {
+                // the stages are free by now: all copies have landed and all MMAs have read them
+                int32_t* part = reinterpret_cast<int32_t*>(smem) + 32 * quad + lane;
+                for (int n = 0; n < it.rows; n += 16) {
+                    int32_t acc[16];
+                    tmem_ld16(d + n, acc);
 #pragma unroll
-                    for (int j = 0; j < 16; ++j) part[(n + j) * kTileM + 32 * quad + lane] = acc[j];
-                } else {
-                    // lane j < 16 fetches column j's output row and scale
-                    int row = 0;
-                    float s = 0.f;
-                    if (n + (lane & 15) < it.rows) {
-                        row = it.first + n + (lane & 15);
-                        if constexpr (GROUPED) row = P.o.order[row];
-                        s = P.o.q_scale[!GROUPED || P.o.per_slot ? row : row / P.o.k];
-                    }
-#pragma unroll
-                    for (int j = 0; j < 16; ++j) {
-                        const int rj = __shfl_sync(0xffffffffu, row, j);
-                        const float sj = __shfl_sync(0xffffffffu, s, j);
-                        if (n + j < it.rows && m < P.o.M) store_y(P.o, rj, m, acc[j], sj, tm);
-                    }
+                    for (int j = 0; j < 16; ++j) part[(n + j) * kTileM] = acc[j];
                 }
+            } else if (P.o.y_type == kTypeF32) {
+                store_tile<float>(P.o, d, it.rows, m, tm, out_row[buf], out_scale[buf]);
+            } else if (P.o.y_type == kTypeF16) {
+                store_tile<__half>(P.o, d, it.rows, m, tm, out_row[buf], out_scale[buf]);
+            } else {
+                store_tile<__nv_bfloat16>(P.o, d, it.rows, m, tm, out_row[buf], out_scale[buf]);
             }
             tc_fence_before();
             __syncwarp();
-            if (lane == 0) mbar_arrive(&acc_free[buf]);
+            if (lane == 0) {
+                if constexpr (PAIR) mbar_arrive_at(&acc_free[buf], 0);
+                else mbar_arrive(&acc_free[buf]);
+            }
         }
+    } else if constexpr (GROUPED) {
+        // ---------------- gathered tokens ----------------
+        // thread x takes 16-byte piece x % 8 of rows x / 8, x / 8 + 16, ..
+        const int x = threadIdx.x - kThreads, piece = x & 7, r0 = x >> 3;
+        constexpr int kRows = (PAIR ? kMaxTileN / 2 : kMaxSingleN) / 16;
+        Ring ring{stages};
+        int filled = 0;
+        bool ok = true;
+        for (int i = item0; i < items && ok; i += item_step) {
+            const Item it = walk.at(i);
+            const int cols = PAIR ? ((it.rows + 31) & ~31) / 2 : (it.rows + 15) & ~15;  // of this CTA, a multiple of 16
+            const int skip = PAIR ? static_cast<int>(rank) * cols : 0;
+            int from[kRows];
+#pragma unroll
+            for (int r = 0; r < kRows; ++r) {
+                if (r * 16 >= cols) break;
+                // what is behind the last row reads that row again
+                const int slot = P.o.order[it.first + min(skip + r0 + 16 * r, it.rows - 1)];
+                from[r] = P.o.per_slot ? slot : slot / P.o.k;
+            }
+            for (int c = c0; c < c1; ++c) {
+                const int s = ring.s;
+                if (filled < stages) ++filled;
+                else if (!mbar_wait(&empty[s], ring.parity ^ 1, 1u, poisoned)) {
+                    ok = false;
+                    break;
+                }
+                // piece p of row r lies at r * 128 + (p ^ (r % 8)) * 16; bytes behind K, where
+                // the weights are zeros, may hold anything, but nothing is read behind the row
+#pragma unroll
+                for (int h = 0; h < kSub; ++h) {
+                    const int k = (c * kSub + h) * kChunk + piece * 16;
+                    const int8_t* src = P.o.q + (k < P.o.K ? k : 0);
+                    const uint32_t bytes = k < P.o.K ? 16 : 0;
+                    const uint32_t dst = smem_u32(smem + s * stage_bytes) + kSub * kABytes + h * b_bytes + r0 * kChunk + ((piece ^ (r0 & 7)) << 4);
+#pragma unroll
+                    for (int r = 0; r < kRows; ++r) {
+                        if (r * 16 >= cols) break;
+                        cp_async16(dst + r * 16 * kChunk, src + from[r] * P.o.q_stride, bytes);
+                    }
+                }
+                cp_async_arrive(&b_full[s]);
+                ring.next();
+            }
+        }
+        asm volatile("cp.async.wait_all;" ::: "memory");
     }
     if constexpr (SPLIT) {
         // one item per cluster, so that the sum over the splits comes after all roles
         __syncwarp();
         cluster_sync();
         if (item0 < items && !*poisoned) {
-            const Item it = item_of<GROUPED>(P, cum, item0);
-            const uint32_t part = smem_u32(smem);
+            const Item it = walk.at(item0);
+            // a warp sums a column's 128 channels, four a lane, over the splits at once
+            const uint32_t part = smem_u32(smem) + 16 * lane;
             const int per = (it.rows + P.splits - 1) / P.splits, n0 = rank * per, n1 = min(n0 + per, it.rows);
-            for (int x = n0 * kTileM + threadIdx.x; x < n1 * kTileM; x += kThreads) {
-                const int n = x / kTileM, m = it.m0 + x % kTileM;
-                if (m >= P.o.M) continue;
-                int32_t acc = 0;
-                for (int r = 0; r < P.splits; ++r) acc += ld_cluster(part + 4 * x, r);
-                int row = it.first + n;
-                if constexpr (GROUPED) row = P.o.order[row];
-                const float s = P.o.q_scale[!GROUPED || P.o.per_slot ? row : row / P.o.k];
-                store_y(P.o, row, m, acc, s, P.o.w_scale[static_cast<int64_t>(it.e) * P.o.M + m]);
+            const int m = it.m0 + 4 * lane;
+            for (int n = n0 + warp; n < n1; n += blockDim.x / 32) {
+                int4 v[8];
+#pragma unroll
+                for (int r = 0; r < 8; ++r)
+                    if (r < P.splits) v[r] = ld_cluster4(part + 4 * kTileM * n, r);
+                int acc[4] = {0, 0, 0, 0};
+#pragma unroll
+                for (int r = 0; r < 8; ++r)
+                    if (r < P.splits) acc[0] += v[r].x, acc[1] += v[r].y, acc[2] += v[r].z, acc[3] += v[r].w;
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    if (m + j < P.o.M)
+                        store_y(P.o, out_row[0][n], m + j,
+                                scaled(acc[j], out_scale[0][n], P.o.w_scale[static_cast<int64_t>(it.e) * P.o.M + m + j]));
             }
         }
-        cluster_sync();  // no CTA ends while another reads its tile
     }
     if constexpr (GROUPED) {
         // slots without an expert come last in the order: their rows are zero
         for (int64_t p = P.o.offsets[P.o.E] + blockIdx.x; p < P.o.slots; p += gridDim.x) {
             const int64_t row = P.o.order[p];
-            for (int m = threadIdx.x; m < P.o.M; m += kThreads) zero_y(P.o, row, m);
+            for (int m = threadIdx.x; m < P.o.M; m += blockDim.x) store_y(P.o, row, m, 0.f);
         }
     }
+    __syncwarp();
     tc_fence_before();
-    __syncthreads();
+    // no CTA ends while another reads its tile or signals its barriers
+    if constexpr (MODE != kSingle) cluster_sync();
+    else __syncthreads();
     tc_fence_after();
-    if (warp == 1)
-        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(P.tmem_cols));
+    if (warp == 1) {
+        if constexpr (PAIR) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(P.tmem_cols));
+        else asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(P.tmem_cols));
+    }
 }
 
 // Rows whose addresses are not multiples of 16 bytes, which the tensor maps
@@ -478,7 +705,7 @@ __global__ void __launch_bounds__(256) i8_general_kernel(const MulMatI8 o) {
             row = o.order[p];
             from = o.per_slot ? row : row / o.k;
             if (p >= o.offsets[o.E]) {
-                if (lane == 0) zero_y(o, row, m);
+                if (lane == 0) store_y(o, row, m, 0.f);
                 continue;
             }
             int hi = o.E - 1;  // the last expert whose first slot is at or before p
@@ -493,7 +720,7 @@ __global__ void __launch_bounds__(256) i8_general_kernel(const MulMatI8 o) {
         int acc = 0;
         for (int k = lane; k < o.K; k += 32) acc += static_cast<int>(w[k]) * q[k];
         acc = __reduce_add_sync(0xffffffffu, acc);
-        if (lane == 0) store_y(o, row, m, acc, o.q_scale[from], o.w_scale[static_cast<int64_t>(e) * o.M + m]);
+        if (lane == 0) store_y(o, row, m, scaled(acc, o.q_scale[from], o.w_scale[static_cast<int64_t>(e) * o.M + m]));
     }
 }
 
@@ -529,13 +756,42 @@ int launch_general(const MulMatI8& o, cudaStream_t stream, int num_sms) {
     return e == cudaSuccess ? 1 : -static_cast<int>(e);
 }
 
-template <bool GROUPED, bool SPLIT>
+template <bool GROUPED, int MODE>
 cudaError_t configure(int dev) {
     static bool done[kMaxDevices] = {};  // the attribute is per device
     if (done[dev]) return cudaSuccess;
-    const cudaError_t e = cudaFuncSetAttribute(i8_kernel<GROUPED, SPLIT>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes);
+    const cudaError_t e = cudaFuncSetAttribute(i8_kernel<GROUPED, MODE>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes);
     done[dev] = e == cudaSuccess;
     return e;
+}
+
+// The mode, the token tile and how many items there are at most.
+struct Plan {
+    Mode mode;
+    int tile_n, splits;
+    int64_t items;
+};
+
+template <bool GROUPED>
+Plan plan(const MulMatI8& o, int num_sms) {
+    Plan p{kSingle, 16, 1, 0};
+    // tokens that a tile should hold: all of them, or an expert's mean share,
+    // doubled (groups are ragged)
+    const int64_t want = GROUPED ? std::min<int64_t>((2 * o.slots + o.E - 1) / o.E, o.slots) : o.N;
+    if (want > kMaxSingleN && o.M > kTileM) p.mode = kPair;
+    const int most = p.mode == kPair ? kMaxTileN : kMaxSingleN, step = p.mode == kPair ? 32 : 16;
+    const int64_t tiles = (want + most - 1) / most;
+    p.tile_n = static_cast<int>(((want + tiles - 1) / tiles + step - 1) / step * step);
+    const int m = p.mode == kPair ? 2 * kTileM : kTileM;
+    const int64_t tiles_m = (o.M + m - 1) / m;
+    // at most one started tile more than the whole ones of each expert
+    const int64_t tiles_n = GROUPED ? std::min<int64_t>(o.slots, o.slots / p.tile_n + o.E) : (o.N + p.tile_n - 1) / p.tile_n;
+    p.items = tiles_n * tiles_m;
+    const int chunks = (o.K + 2 * kChunk - 1) / (2 * kChunk);
+    if (p.mode == kSingle)
+        while (p.splits < 8 && p.items * p.splits * 2 <= num_sms && chunks >= p.splits * 2) p.splits *= 2;
+    if (p.splits > 1) p.mode = kSplit;
+    return p;
 }
 
 template <bool GROUPED>
@@ -548,26 +804,17 @@ int launch(const MulMatI8& o, cudaStream_t stream, int num_sms) {
     if (const cudaError_t e = cudaGetDevice(&dev); e != cudaSuccess) return -static_cast<int>(e);
     if (dev < 0 || dev >= kMaxDevices) return -static_cast<int>(cudaErrorInvalidDevice);
 
+    const Plan plan = wllm::plan<GROUPED>(o, num_sms);
+    if (plan.items > 0x7fffffff) return -static_cast<int>(cudaErrorInvalidValue);
     I8Args P{};
     P.o = o;
-    P.tiles_m = (o.M + kTileM - 1) / kTileM;
-    P.chunks = (o.K + kChunk - 1) / kChunk;
-    // tokens of a tile, and how many items there are at most
-    int64_t items;
-    if (GROUPED) {
-        // an expert's mean share, doubled (groups are ragged), in tiles of at most 256
-        const int64_t mean = (2 * o.slots + o.E - 1) / o.E;
-        P.tile_n = static_cast<int>(std::min<int64_t>(kMaxTileN, std::min<int64_t>((mean + 15) / 16 * 16, (o.slots + 15) / 16 * 16)));
-        items = std::min<int64_t>(o.slots, o.slots / P.tile_n + o.E) * P.tiles_m;
-    } else {
-        const int tiles = (o.N + kMaxTileN - 1) / kMaxTileN;
-        P.tile_n = ((o.N + tiles - 1) / tiles + 15) / 16 * 16;
-        items = static_cast<int64_t>((o.N + P.tile_n - 1) / P.tile_n) * P.tiles_m;
-    }
-    P.splits = 1;
-    if (P.tile_n <= 64)
-        while (P.splits < 8 && items * P.splits * 2 <= num_sms && P.chunks >= P.splits * 4) P.splits *= 2;
-    const int stage_bytes = kABytes + P.tile_n * kChunk;
+    P.tile_n = plan.tile_n;
+    P.splits = plan.splits;
+    P.tiles_m = (o.M + (plan.mode == kPair ? 2 : 1) * kTileM - 1) / ((plan.mode == kPair ? 2 : 1) * kTileM);
+    const int sub = plan.mode == kPair ? chunks_of_stage<kPair>() : chunks_of_stage<kSingle>();
+    P.chunks = (o.K + sub * kChunk - 1) / (sub * kChunk);
+    const int tokens = plan.mode == kPair ? P.tile_n / 2 : P.tile_n;  // of a CTA's stage
+    const int stage_bytes = sub * (kABytes + tokens * kChunk);
     P.stages = std::min(kMaxStages, (kSmemBytes - 1024) / stage_bytes);
     P.tmem_cols = 32;
     while (P.tmem_cols < 2 * P.tile_n) P.tmem_cols *= 2;
@@ -577,28 +824,32 @@ int launch(const MulMatI8& o, cudaStream_t stream, int num_sms) {
                                        static_cast<cuuint64_t>(o.E > 1 ? o.w_expert_bytes : o.w_row_bytes * o.M)};
         if (!encode(&P.wmap, o.w, 3, dims, strides, kTileM)) return -static_cast<int>(cudaErrorInvalidValue);
     }
-    {
+    if (!GROUPED) {
         const cuuint64_t dims[2] = {static_cast<cuuint64_t>(o.K), static_cast<cuuint64_t>(o.N)};
         const cuuint64_t strides[1] = {static_cast<cuuint64_t>(o.q_stride)};
-        if (!encode(&P.xmap, o.q, 2, dims, strides, GROUPED ? 1 : P.tile_n)) return -static_cast<int>(cudaErrorInvalidValue);
+        if (!encode(&P.xmap, o.q, 2, dims, strides, tokens)) return -static_cast<int>(cudaErrorInvalidValue);
     }
-    const bool split = P.splits > 1;
-    if (const cudaError_t e = split ? configure<GROUPED, true>(dev) : configure<GROUPED, false>(dev); e != cudaSuccess)
-        return -static_cast<int>(e);
+    void (*const kernels[3])(I8Args) = {i8_kernel<GROUPED, kSingle>, i8_kernel<GROUPED, kSplit>, i8_kernel<GROUPED, kPair>};
+    const cudaError_t set = plan.mode == kSingle  ? configure<GROUPED, kSingle>(dev)
+                            : plan.mode == kSplit ? configure<GROUPED, kSplit>(dev)
+                                                  : configure<GROUPED, kPair>(dev);
+    if (set != cudaSuccess) return -static_cast<int>(set);
+    const int group = plan.mode == kPair ? 2 : P.splits;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(static_cast<unsigned>(split ? items * P.splits : std::min<int64_t>(items, num_sms)));
-    cfg.blockDim = dim3(kThreads);
+    cfg.gridDim = dim3(static_cast<unsigned>(
+        plan.mode == kSplit ? plan.items * group : std::min<int64_t>(plan.items, num_sms / group) * group));
+    cfg.blockDim = dim3(GROUPED ? kThreads + kLoaders : kThreads);
     cfg.dynamicSmemBytes = 1024 + P.stages * stage_bytes;
     cfg.stream = stream;
     cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     attr[1].id = cudaLaunchAttributeClusterDimension;
-    attr[1].val.clusterDim.x = static_cast<unsigned>(P.splits);
+    attr[1].val.clusterDim.x = static_cast<unsigned>(group);
     attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
     cfg.attrs = attr;
-    cfg.numAttrs = split ? 2 : 1;
-    const cudaError_t e = cudaLaunchKernelEx(&cfg, split ? i8_kernel<GROUPED, true> : i8_kernel<GROUPED, false>, P);
+    cfg.numAttrs = group > 1 ? 2 : 1;
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, kernels[plan.mode], P);
     return e == cudaSuccess ? 1 : -static_cast<int>(e);
 }
 
