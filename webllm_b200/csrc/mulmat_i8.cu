@@ -60,14 +60,10 @@ namespace {
 
 constexpr int kTileM = 128;    // channels of a tile
 constexpr int kMaxTileN = 256; // tokens of a pair's tile
+constexpr int kMaxShortN = 128; // of a pair's with two chunks a stage
 constexpr int kMaxSingleN = 64; // of a single CTA's or a split one
 constexpr int kChunk = 128;    // bytes of K of a swizzled row
 constexpr int kABytes = kTileM * kChunk;
-// Chunks of a stage. A stage costs its copy and MMA warps some 350 clocks of
-// waits and issue whatever its size; the 256-token MMAs of a pair's chunk take
-// 512, those of a single token far less, so there two chunks share a stage.
-template <int MODE>
-__host__ __device__ constexpr int chunks_of_stage();
 constexpr int kThreads = 192;       // copies, MMAs, four epilogue warps
 constexpr int kLoaders = 128;       // threads that gather tokens
 constexpr int kMaxStages = 12;
@@ -84,9 +80,13 @@ struct I8Args {
     int32_t tmem_cols;
 };
 
-enum Mode : int { kSingle = 0, kSplit = 1, kPair = 2 };
-template <int MODE>
-__host__ __device__ constexpr int chunks_of_stage() { return MODE == kPair ? 1 : 2; }
+enum Mode : int { kSingle = 0, kSplit = 1, kPair = 2, kPairShort = 3 };
+// Chunks of a stage. A stage costs its copy and MMA warps some 350 clocks of
+// waits and issue whatever its size; the MMAs of a pair's chunk with 256 tokens
+// take 512, those of fewer tokens less, so there (kPairShort: at most 128
+// tokens) two chunks share a stage.
+__host__ __device__ constexpr int chunks_of_stage(int mode) { return mode == kPair ? 1 : 2; }
+__host__ __device__ constexpr bool is_pair(int mode) { return mode >= kPair; }
 
 __device__ __forceinline__ uint32_t smem_u32(const void* p) { return static_cast<uint32_t>(__cvta_generic_to_shared(p)); }
 __device__ __forceinline__ void mbar_init(uint64_t* bar, uint32_t count) {
@@ -160,11 +160,15 @@ __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, uint32
 __device__ __forceinline__ void cp_async_arrive(uint64_t* bar) {
     asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
 }
-// Arrives on the barrier at bar's place in CTA `rank` of the cluster.
+// Arrives on the barrier at bar's place in CTA `rank` of the cluster. What it
+// orders is not memory that the other CTA's threads read, but the tensor pipe's
+// operands (fenced for its proxy by the caller) and accumulators. (Released at
+// cluster scope the arrive waits for the thread's global stores: 1500 clocks a
+// chunk, 144 us against 64 for 512 tokens in 8 of 64 experts, 2048 -> 2048.)
 __device__ __forceinline__ void mbar_arrive_at(uint64_t* bar, uint32_t rank) {
     uint32_t remote;
     asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(smem_u32(bar)), "r"(rank));
-    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(remote) : "memory");
+    asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(remote) : "memory");
 }
 __device__ __forceinline__ void fence_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 __device__ __forceinline__ void tma_prefetch_3d(const CUtensorMap* tm, int x, int y, int z) {
@@ -244,6 +248,10 @@ struct Ring {
 __device__ __forceinline__ void cluster_sync() {
     asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
+// The same without ordering memory (global stores before it are not waited for).
+__device__ __forceinline__ void cluster_meet() {
+    asm volatile("barrier.cluster.arrive.relaxed.aligned;\n\tbarrier.cluster.wait.aligned;" ::: "memory");
+}
 __device__ __forceinline__ int4 ld_cluster4(uint32_t local, uint32_t rank) {
     uint32_t remote;
     int4 v;
@@ -286,8 +294,8 @@ struct Walk {
     int e = 0;
 
     __device__ __forceinline__ Item at(int i) {
-        constexpr int kM = MODE == kPair ? 2 * kTileM : kTileM;
-        constexpr int kStep = MODE == kPair ? 32 : 16;
+        constexpr int kM = is_pair(MODE) ? 2 * kTileM : kTileM;
+        constexpr int kStep = is_pair(MODE) ? 32 : 16;
         Item it;
         if constexpr (!GROUPED) {
             const int tiles = (P.o.N + P.tile_n - 1) / P.tile_n;
@@ -335,21 +343,22 @@ __device__ __forceinline__ void store_tile(const MulMatI8& o, uint32_t taddr, in
 
 template <bool GROUPED, int MODE>
 __global__ void __launch_bounds__(GROUPED ? kThreads + kLoaders : kThreads, 1) i8_kernel(const __grid_constant__ I8Args P) {
-    constexpr bool SPLIT = MODE == kSplit, PAIR = MODE == kPair;
+    constexpr bool SPLIT = MODE == kSplit, PAIR = is_pair(MODE);
+    constexpr int kTokens = MODE == kPair ? kMaxTileN : (PAIR ? kMaxShortN : kMaxSingleN);
     extern __shared__ __align__(1024) uint8_t smem_raw[];
     __shared__ uint64_t full[kMaxStages], b_full[kMaxStages], empty[kMaxStages], acc_full[2], acc_free[2];
     __shared__ uint32_t tmem_slot;
     __shared__ int poison;
     __shared__ int32_t cum[GROUPED ? kMaxExperts + 1 : 1], begin[GROUPED ? kMaxExperts + 1 : 1];
     __shared__ int32_t warp_sum[10];
-    __shared__ int32_t out_row[2][PAIR ? kMaxTileN : kMaxSingleN];
-    __shared__ float out_scale[2][PAIR ? kMaxTileN : kMaxSingleN];
+    __shared__ int32_t out_row[2][kTokens];
+    __shared__ float out_scale[2][kTokens];
     // 1024-byte alignment for the swizzled tiles
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     volatile int* poisoned = &poison;
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    constexpr int kSub = chunks_of_stage<MODE>();
+    constexpr int kSub = chunks_of_stage(MODE);
     const int stages = P.stages, b_bytes = (PAIR ? P.tile_n / 2 : P.tile_n) * kChunk;
     const int stage_bytes = kSub * (kABytes + b_bytes);  // kSub weight chunks, then as many of the tokens
     uint32_t rank = 0;  // in the cluster
@@ -598,7 +607,7 @@ __global__ void __launch_bounds__(GROUPED ? kThreads + kLoaders : kThreads, 1) i
         // ---------------- gathered tokens ----------------
         // thread x takes 16-byte piece x % 8 of rows x / 8, x / 8 + 16, ..
         const int x = threadIdx.x - kThreads, piece = x & 7, r0 = x >> 3;
-        constexpr int kRows = (PAIR ? kMaxTileN / 2 : kMaxSingleN) / 16;
+        constexpr int kRows = (PAIR ? kTokens / 2 : kTokens) / 16;
         Ring ring{stages};
         int filled = 0;
         bool ok = true;
@@ -678,7 +687,7 @@ __global__ void __launch_bounds__(GROUPED ? kThreads + kLoaders : kThreads, 1) i
     __syncwarp();
     tc_fence_before();
     // no CTA ends while another reads its tile or signals its barriers
-    if constexpr (MODE != kSingle) cluster_sync();
+    if constexpr (MODE != kSingle) cluster_meet();
     else __syncthreads();
     tc_fence_after();
     if (warp == 1) {
@@ -756,15 +765,6 @@ int launch_general(const MulMatI8& o, cudaStream_t stream, int num_sms) {
     return e == cudaSuccess ? 1 : -static_cast<int>(e);
 }
 
-template <bool GROUPED, int MODE>
-cudaError_t configure(int dev) {
-    static bool done[kMaxDevices] = {};  // the attribute is per device
-    if (done[dev]) return cudaSuccess;
-    const cudaError_t e = cudaFuncSetAttribute(i8_kernel<GROUPED, MODE>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes);
-    done[dev] = e == cudaSuccess;
-    return e;
-}
-
 // The mode, the token tile and how many items there are at most.
 struct Plan {
     Mode mode;
@@ -778,11 +778,12 @@ Plan plan(const MulMatI8& o, int num_sms) {
     // tokens that a tile should hold: all of them, or an expert's mean share,
     // doubled (groups are ragged)
     const int64_t want = GROUPED ? std::min<int64_t>((2 * o.slots + o.E - 1) / o.E, o.slots) : o.N;
-    if (want > kMaxSingleN && o.M > kTileM) p.mode = kPair;
-    const int most = p.mode == kPair ? kMaxTileN : kMaxSingleN, step = p.mode == kPair ? 32 : 16;
+    if (want > kMaxSingleN && o.M > kTileM) p.mode = want <= kMaxShortN ? kPairShort : kPair;
+    const bool pair = is_pair(p.mode);
+    const int most = pair ? kMaxTileN : kMaxSingleN, step = pair ? 32 : 16;
     const int64_t tiles = (want + most - 1) / most;
     p.tile_n = static_cast<int>(((want + tiles - 1) / tiles + step - 1) / step * step);
-    const int m = p.mode == kPair ? 2 * kTileM : kTileM;
+    const int m = pair ? 2 * kTileM : kTileM;
     const int64_t tiles_m = (o.M + m - 1) / m;
     // at most one started tile more than the whole ones of each expert
     const int64_t tiles_n = GROUPED ? std::min<int64_t>(o.slots, o.slots / p.tile_n + o.E) : (o.N + p.tile_n - 1) / p.tile_n;
@@ -791,6 +792,7 @@ Plan plan(const MulMatI8& o, int num_sms) {
     if (p.mode == kSingle)
         while (p.splits < 8 && p.items * p.splits * 2 <= num_sms && chunks >= p.splits * 2) p.splits *= 2;
     if (p.splits > 1) p.mode = kSplit;
+    if (pair && p.tile_n <= kMaxShortN) p.mode = kPairShort;
     return p;
 }
 
@@ -810,10 +812,11 @@ int launch(const MulMatI8& o, cudaStream_t stream, int num_sms) {
     P.o = o;
     P.tile_n = plan.tile_n;
     P.splits = plan.splits;
-    P.tiles_m = (o.M + (plan.mode == kPair ? 2 : 1) * kTileM - 1) / ((plan.mode == kPair ? 2 : 1) * kTileM);
-    const int sub = plan.mode == kPair ? chunks_of_stage<kPair>() : chunks_of_stage<kSingle>();
+    const bool pair = is_pair(plan.mode);
+    const int tile_m = pair ? 2 * kTileM : kTileM, sub = chunks_of_stage(plan.mode);
+    P.tiles_m = (o.M + tile_m - 1) / tile_m;
     P.chunks = (o.K + sub * kChunk - 1) / (sub * kChunk);
-    const int tokens = plan.mode == kPair ? P.tile_n / 2 : P.tile_n;  // of a CTA's stage
+    const int tokens = pair ? P.tile_n / 2 : P.tile_n;  // of a CTA's stage
     const int stage_bytes = sub * (kABytes + tokens * kChunk);
     P.stages = std::min(kMaxStages, (kSmemBytes - 1024) / stage_bytes);
     P.tmem_cols = 32;
@@ -829,12 +832,15 @@ int launch(const MulMatI8& o, cudaStream_t stream, int num_sms) {
         const cuuint64_t strides[1] = {static_cast<cuuint64_t>(o.q_stride)};
         if (!encode(&P.xmap, o.q, 2, dims, strides, tokens)) return -static_cast<int>(cudaErrorInvalidValue);
     }
-    void (*const kernels[3])(I8Args) = {i8_kernel<GROUPED, kSingle>, i8_kernel<GROUPED, kSplit>, i8_kernel<GROUPED, kPair>};
-    const cudaError_t set = plan.mode == kSingle  ? configure<GROUPED, kSingle>(dev)
-                            : plan.mode == kSplit ? configure<GROUPED, kSplit>(dev)
-                                                  : configure<GROUPED, kPair>(dev);
-    if (set != cudaSuccess) return -static_cast<int>(set);
-    const int group = plan.mode == kPair ? 2 : P.splits;
+    void (*const kernels[4])(I8Args) = {i8_kernel<GROUPED, kSingle>, i8_kernel<GROUPED, kSplit>, i8_kernel<GROUPED, kPair>,
+                                        i8_kernel<GROUPED, kPairShort>};
+    static bool configured[kMaxDevices][4] = {};  // the attribute is per device
+    if (!configured[dev][plan.mode]) {
+        const cudaError_t e = cudaFuncSetAttribute(kernels[plan.mode], cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes);
+        if (e != cudaSuccess) return -static_cast<int>(e);
+        configured[dev][plan.mode] = true;
+    }
+    const int group = pair ? 2 : P.splits;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(static_cast<unsigned>(
         plan.mode == kSplit ? plan.items * group : std::min<int64_t>(plan.items, num_sms / group) * group));
