@@ -5,21 +5,24 @@
 //
 // v is the row itself, RMS_NORM(x) * gain, or act(gate) * up. Ties go to the
 // even integer and the quotient is the exact one, so q does not depend on how
-// a division is rounded: t = v * (1/s) is within 127 * 2^-22 of the quotient,
-// so only a t within 1/10000 of a half can round to the wrong integer, and
-// there the remainder r = v - q s decides (one FMA; where 2|r| is near s it
-// has at most 24 bits, so it is exact, and FMA's rounding is monotone
-// elsewhere). A row whose a is below 2^-100, where 1/s could overflow, or
-// s be rounded to a few bits, takes double quotients, clamped to +-127.
+// a division is rounded: v is multiplied by 1/s once a little too small and
+// once a little too large, each product and its rounding to an integer one FMA
+// (two values an instruction), and only where the two integers differ the
+// remainder r = v - q s decides (one FMA; where 2|r| is near s it has at most
+// 24 bits, so it is exact, and FMA's rounding is monotone elsewhere). Of f32
+// values that is 3 in 100,000; of bf16 ones, whose quotients 127 v / a are ratios
+// of small numbers, one in some hundred is an exact tie. A row whose a is below
+// 2^-100, where 1/s could overflow or s be rounded to a few bits, takes double
+// quotients, clamped to +-127.
 // A row that holds a NaN or an infinity has no scale: s = NaN and q = 0, so
 // every product of it is NaN.
 //
 // Bound: HBM (one read of the row, K + 4 bytes written). One CTA per row; the
-// row's values stay in registers (32 a thread) between the maximum and the
-// rounding, so rows up to 32 * 512 values are read once; longer rows are read
-// again (from L2) in the second pass.
+// row's values stay in registers between the maximum and the rounding, so rows
+// up to 32 values a thread are read once; longer rows are read again (from L2)
+// in the second pass.
 // Threads: rows that are few take one 8-value vector a thread (latency), many
-// rows four (fewer barriers a byte).
+// rows as many as its registers keep (fewer barriers a byte).
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <stdint.h>
@@ -33,7 +36,9 @@ namespace wllm {
 namespace {
 
 constexpr int kVec = 8;    // values of a thread's vector
-constexpr int kKeep = 4;   // vectors a thread keeps in registers
+// Vectors a thread keeps in registers: 32 of them, as loaded or (with a
+// prologue) as f32.
+__host__ __device__ constexpr int keep_vecs(int size, int pro) { return size == 2 && pro == kProNone ? 8 : 4; }
 constexpr int kMaxThreads = 512;
 constexpr int kFewRows = 512;  // at most this many rows: one vector a thread
 
@@ -62,32 +67,32 @@ __device__ __forceinline__ void unpack(const Raw<T>& r, float (&v)[kVec]) {
     }
 }
 
-// Values [8 i, 8 i + 8) of a row, zeros behind its end. VEC: the row starts on
-// a 16-byte boundary.
+// Values [8 i, 8 i + 8) of a row. VEC: the row starts on a 16-byte boundary.
 template <typename T, bool VEC>
-__device__ __forceinline__ Raw<T> load_part(const T* row, int i, int K) {
+__device__ __forceinline__ Raw<T> load_vec(const T* row, int i) {
     Raw<T> r;
-    if (VEC && (i + 1) * kVec <= K) {
+    if constexpr (VEC) {
         const uint4* p = reinterpret_cast<const uint4*>(row + static_cast<int64_t>(i) * kVec);
 #pragma unroll
         for (int h = 0; h < Raw<T>::kWords / 4; ++h) {
             const uint4 a = p[h];
             r.w[4 * h] = a.x, r.w[4 * h + 1] = a.y, r.w[4 * h + 2] = a.z, r.w[4 * h + 3] = a.w;
         }
+    } else if constexpr (sizeof(T) == 4) {
+#pragma unroll
+        for (int j = 0; j < kVec; ++j) r.w[j] = reinterpret_cast<const uint32_t*>(row)[static_cast<int64_t>(i) * kVec + j];
     } else {
-        using U = typename std::conditional<sizeof(T) == 4, uint32_t, uint16_t>::type;
-        const U* p = reinterpret_cast<const U*>(row);
+        const uint16_t* p = reinterpret_cast<const uint16_t*>(row) + static_cast<int64_t>(i) * kVec;
 #pragma unroll
-        for (int h = 0; h < Raw<T>::kWords; ++h) {
-            r.w[h] = 0;
-#pragma unroll
-            for (int j = 0; j < 4 / static_cast<int>(sizeof(T)); ++j) {
-                const int k = i * kVec + h * (4 / static_cast<int>(sizeof(T))) + j;
-                if (k < K) r.w[h] |= static_cast<uint32_t>(p[k]) << (16 * j);
-            }
-        }
+        for (int h = 0; h < kVec / 2; ++h) r.w[h] = p[2 * h] | static_cast<uint32_t>(p[2 * h + 1]) << 16;
     }
     return r;
+}
+template <typename T>
+__device__ __forceinline__ float to_f32(T v) {
+    if constexpr (sizeof(T) == 4) return v;
+    else if constexpr (std::is_same<T, __half>::value) return __half2float(v);
+    else return __bfloat162float(v);
 }
 
 // The largest |value| of vectors so far. The bits of |v| order like its value,
@@ -110,8 +115,16 @@ __device__ __forceinline__ uint32_t top_bits(uint32_t top) {
     return h << 16;
 }
 
-// silu(g) * u and gelu(g) * u, as wllm_mul_mat_glu_batch computes them
-__device__ __forceinline__ float x_sigmoid(float x, float z) { return __fdividef(x, 1.f + __expf(-z)); }
+// silu(g) * u and gelu(g) * u, as wllm_mul_mat_glu_batch computes them: x / (1 +
+// e^-z) with the SFU's exponential and reciprocal. What they flush to zero (an
+// e^-z below 2^-126, a reciprocal of more than 2^126) is lost in the sum or the
+// product anyway.
+__device__ __forceinline__ float x_sigmoid(float x, float z) {
+    float e, r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(z * -1.4426950408889634f));
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.f + e));
+    return x * r;
+}
 __device__ __forceinline__ float glu(int kind, float g, float u) {
     if (kind == kProSwiglu) return __fmul_rn(x_sigmoid(g, g), u);
     float y;
@@ -147,197 +160,215 @@ __device__ __forceinline__ float block_sum(float v, float* part) {
     return v;
 }
 
-// The nearest integer to v / s where t = v * (1/s) is too near a half to tell.
-__device__ __forceinline__ float settle(float v, float s, float q) {
-    const float r = 2.f * fmaf(-q, s, v);
-    const bool odd = static_cast<int>(q) & 1;
-    if (r > s || (r == s && odd)) return q + 1.f;
-    if (r < -s || (r == -s && odd)) return q - 1.f;
-    return q;
+__device__ __forceinline__ uint64_t pack2(float a, float b) {
+    return static_cast<uint64_t>(__float_as_uint(b)) << 32 | __float_as_uint(a);
 }
-// The same in a row of tiny values.
-__device__ __noinline__ float settle_tiny(float v, float s) {
-    return s > 0.f ? static_cast<float>(fmin(fmax(rint(static_cast<double>(v) / s), -127.0), 127.0)) : 0.f;
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+    return d;
+}
+
+constexpr float kMagic = 12582912.f;  // 1.5 * 2^23: a sum with it is rounded to the nearest integer (ties to even)
+
+// A row's scale and what its values are multiplied by: 1/s a little too small
+// and a little too large (by 2^-21, where 1/s is off by 2^-24).
+struct Scale {
+    float s, lo, hi;
+};
+
+// Of the integers (as sums with kMagic) that v * lo and v * hi round to, the
+// nearest to v / s; where they differ the remainder of the smaller decides.
+__device__ __forceinline__ uint32_t nearest(float v, float s, uint32_t lo, uint32_t hi) {
+    const float r = fabsf(2.f * fmaf(-(__uint_as_float(lo) - kMagic), s, v));
+    return r > s || (r == s && (lo & 1)) ? hi : lo;
+}
+__device__ __forceinline__ int8_t quantize1(float v, const Scale& c) {
+    return static_cast<int8_t>(nearest(v, c.s, __float_as_uint(fmaf(v, c.lo, kMagic)), __float_as_uint(fmaf(v, c.hi, kMagic))));
+}
+// In a row of tiny values, where 1/s could overflow.
+__device__ __forceinline__ int8_t quantize_tiny(float v, float s) {
+    return s > 0.f ? static_cast<int8_t>(fmin(fmax(rint(static_cast<double>(v) / s), -127.0), 127.0)) : 0;
 }
 
 // Eight int8 of a vector.
-__device__ __forceinline__ uint2 quantize8(const float (&v)[kVec], float s, float inv, bool tiny) {
-    constexpr float kMagic = 12582912.f;  // 1.5 * 2^23: adding it rounds to the nearest integer (ties to even)
-    float m[kVec];
-    float worst = 0.f;
+__device__ __forceinline__ uint2 quantize8(const float (&v)[kVec], const Scale& c) {
+    const uint64_t magic = pack2(kMagic, kMagic), lo = pack2(c.lo, c.lo), hi = pack2(c.hi, c.hi);
+    uint32_t m[kVec], n[kVec], apart = 0;
 #pragma unroll
-    for (int j = 0; j < kVec; ++j) {
-        const float t = v[j] * inv;
-        m[j] = __fadd_rn(t, kMagic);
-        worst = fmaxf(worst, fabsf(t - (m[j] - kMagic)));
+    for (int j = 0; j < kVec; j += 2) {
+        const uint64_t p = pack2(v[j], v[j + 1]);
+        const uint64_t a = fma2(p, lo, magic), b = fma2(p, hi, magic);
+        m[j] = static_cast<uint32_t>(a), m[j + 1] = static_cast<uint32_t>(a >> 32);
+        n[j] = static_cast<uint32_t>(b), n[j + 1] = static_cast<uint32_t>(b >> 32);
+        apart |= (m[j] ^ n[j]) | (m[j + 1] ^ n[j + 1]);
     }
-    if (worst > 0.4999f) {
+    if (apart) {
 #pragma unroll
-        for (int j = 0; j < kVec; ++j) m[j] = settle(v[j], s, m[j] - kMagic) + kMagic;
-    }
-    if (tiny) {
-#pragma unroll
-        for (int j = 0; j < kVec; ++j) m[j] = settle_tiny(v[j], s) + kMagic;
+        for (int j = 0; j < kVec; ++j) m[j] = nearest(v[j], c.s, m[j], n[j]);
     }
     uint32_t w[2];
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-        const uint32_t a = __byte_perm(__float_as_uint(m[4 * h]), __float_as_uint(m[4 * h + 1]), 0x0040);
-        const uint32_t b = __byte_perm(__float_as_uint(m[4 * h + 2]), __float_as_uint(m[4 * h + 3]), 0x0040);
-        w[h] = __byte_perm(a, b, 0x5410);
-    }
+    for (int h = 0; h < 2; ++h)
+        w[h] = __byte_perm(__byte_perm(m[4 * h], m[4 * h + 1], 0x0040), __byte_perm(m[4 * h + 2], m[4 * h + 3], 0x0040), 0x5410);
     return make_uint2(w[0], w[1]);
 }
 
 // PRO: kProNone, kProNorm, or kProSwiglu for both GLU kinds (P.kind tells).
-// Without a prologue the kept vectors stay as they were loaded (16 registers
-// of a 16-bit type), so three CTAs of 512 threads fit an SM (two of f32 or with
-// a prologue): at one CTA the loads of the next row do not overlap the rounding
-// of this one (8192 x 14336 bf16: 223 us against 62).
+// VEC: rows of x and up start on 16-byte boundaries, rows of q on 8-byte ones.
+// At 64 registers and some 114 KB of a full SM's loads in flight, the loads of
+// other rows run while one is rounded.
 template <typename T, bool VEC, int PRO>
-__global__ void __launch_bounds__(kMaxThreads, PRO == kProNone && sizeof(T) == 2 ? 3 : 2) quantize_i8_kernel(const QuantizeI8 P) {
+__global__ void __launch_bounds__(kMaxThreads, 2) quantize_i8_kernel(const QuantizeI8 P) {
+    constexpr int kKeep = keep_vecs(sizeof(T), PRO);
     __shared__ uint32_t part_max[kMaxThreads / 32];
     __shared__ float part_sum[kMaxThreads / 32];
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     asm volatile("griddepcontrol.wait;" ::: "memory");
     const int64_t r = blockIdx.x;
     const T* x = static_cast<const T*>(P.x) + r * P.x_stride;
-    const int K = P.K, parts = (K + kVec - 1) / kVec;
-    const int step = blockDim.x;
-    float rms = 1.f;
-    uint32_t top = 0;
-
-    // s, 1/s and the stores are the same for every prologue
-    float s = 0.f, inv = 0.f;
-    bool bad = false, tiny = false;
-    auto set_scale = [&]() {
-        top = block_max(top, part_max);
-        bad = top >= 0x7f800000u;
-        const float a = __uint_as_float(top);
-        s = bad ? __uint_as_float(0x7fc00000u) : __fdiv_rn(a, 127.f);
-        tiny = a < 0x1p-100f;
-        inv = bad || tiny ? 0.f : __fdiv_rn(1.f, s);
-        if (threadIdx.x == 0) P.scale[r] = s;
-    };
+    const T* up = PRO == kProSwiglu ? static_cast<const T*>(P.up) + r * P.up_stride : nullptr;
     int8_t* q = P.q + r * P.q_stride;
-    const bool wide = ((reinterpret_cast<uintptr_t>(P.q) | static_cast<uintptr_t>(P.q_stride)) & 7) == 0;
-    auto store = [&](int i, float (&v)[kVec]) {
-        uint2 w = quantize8(v, s, inv, tiny);
-        if (bad) w = make_uint2(0, 0);
-        if (wide && (i + 1) * kVec <= K) {
+    const int K = P.K, vecs = K / kVec, step = blockDim.x;  // whole vectors; up to 7 values behind them
+    float rms = 1.f;
+
+    // the prologue on a vector's or a single value
+    auto value = [&](const Raw<T>& a, const Raw<T>& b, float (&v)[kVec]) {
+        unpack<T>(a, v);
+        if constexpr (PRO == kProSwiglu) {
+            float u[kVec];
+            unpack<T>(b, u);
+#pragma unroll
+            for (int j = 0; j < kVec; ++j) v[j] = glu(P.kind, v[j], u[j]);
+        }
+    };
+    auto value_at = [&](int i, float (&v)[kVec]) {
+        const Raw<T> a = load_vec<T, VEC>(x, i);
+        value(a, PRO == kProSwiglu ? load_vec<T, VEC>(up, i) : a, v);
+    };
+    auto scaled = [&](int k, float v) {
+        if constexpr (PRO == kProNorm) {
+            v = __fmul_rn(v, rms);
+            if (P.gain) v = __fmul_rn(v, P.gain[k]);
+        }
+        return v;
+    };
+    auto scaled_vec = [&](int i, float (&v)[kVec]) {
+#pragma unroll
+        for (int j = 0; j < kVec; ++j) v[j] = scaled(i * kVec + j, v[j]);
+    };
+    auto single = [&](int k) {
+        const float v = to_f32(x[k]);
+        return PRO == kProSwiglu ? glu(P.kind, v, to_f32(up[k])) : v;
+    };
+    auto bits = [](float v) { return __float_as_uint(v) & 0x7fffffffu; };
+    auto max_vec = [&](uint32_t top, const float (&v)[kVec]) {
+#pragma unroll
+        for (int j = 0; j < kVec; ++j) top = max(top, bits(v[j]));
+        return top;
+    };
+    auto store = [&](int i, const float (&v)[kVec], const Scale& c) {
+        const uint2 w = quantize8(v, c);
+        if constexpr (VEC) {
             *reinterpret_cast<uint2*>(q + static_cast<int64_t>(i) * kVec) = w;
         } else {
-            const uint64_t b = (static_cast<uint64_t>(w.y) << 32) | w.x;
-            for (int j = 0; j < kVec && i * kVec + j < K; ++j) q[i * kVec + j] = static_cast<int8_t>(b >> (8 * j));
+#pragma unroll
+            for (int j = 0; j < kVec; ++j)
+                q[static_cast<int64_t>(i) * kVec + j] = static_cast<int8_t>((j < 4 ? w.x : w.y) >> (8 * (j & 3)));
         }
     };
 
+    // ---- into registers (all loads of the kept vectors in flight together), and the maximum
+    uint32_t top = 0;
+    Raw<T> raw[PRO == kProNone ? kKeep : 1];
+    float keep[PRO == kProNone ? 1 : kKeep][kVec];
     if constexpr (PRO == kProNone) {
-        Raw<T> keep[kKeep];
 #pragma unroll
         for (int c = 0; c < kKeep; ++c) {
             const int i = threadIdx.x + c * step;
-            if (i < parts) keep[c] = load_part<T, VEC>(x, i, K);
+            if (i < vecs) raw[c] = load_vec<T, VEC>(x, i);
             else
 #pragma unroll
-                for (int h = 0; h < Raw<T>::kWords; ++h) keep[c].w[h] = 0;
+                for (int h = 0; h < Raw<T>::kWords; ++h) raw[c].w[h] = 0;
         }
 #pragma unroll
-        for (int c = 0; c < kKeep; ++c) top = max_raw<T>(top, keep[c]);
-        for (int i = threadIdx.x + kKeep * step; i < parts; i += step) top = max_raw<T>(top, load_part<T, VEC>(x, i, K));
+        for (int c = 0; c < kKeep; ++c) top = max_raw<T>(top, raw[c]);
+        for (int i = threadIdx.x + kKeep * step; i < vecs; i += step) top = max_raw<T>(top, load_vec<T, VEC>(x, i));
         top = top_bits<T>(top);
-        set_scale();
-#pragma unroll
-        for (int c = 0; c < kKeep; ++c) {
-            const int i = threadIdx.x + c * step;
-            if (i < parts) {
-                float v[kVec];
-                unpack<T>(keep[c], v);
-                store(i, v);
-            }
-        }
-        for (int i = threadIdx.x + kKeep * step; i < parts; i += step) {
-            float v[kVec];
-            unpack<T>(load_part<T, VEC>(x, i, K), v);
-            store(i, v);
-        }
     } else {
-        const T* up = PRO == kProSwiglu ? static_cast<const T*>(P.up) + r * P.up_stride : nullptr;
-        float keep[kKeep][kVec];
-        auto value = [&](const Raw<T>& a, const Raw<T>& b, float (&v)[kVec]) {
-            unpack<T>(a, v);
-            if constexpr (PRO == kProSwiglu) {
-                float u[kVec];
-                unpack<T>(b, u);
-#pragma unroll
-                for (int j = 0; j < kVec; ++j) v[j] = glu(P.kind, v[j], u[j]);
-            }
-        };
-        auto value_at = [&](int i, float (&v)[kVec]) {
-            const Raw<T> a = load_part<T, VEC>(x, i, K);
-            value(a, PRO == kProSwiglu ? load_part<T, VEC>(up, i, K) : a, v);
-        };
-        auto scaled = [&](int i, float (&v)[kVec]) {
-            if constexpr (PRO == kProNorm) {
-#pragma unroll
-                for (int j = 0; j < kVec; ++j) {
-                    v[j] = __fmul_rn(v[j], rms);
-                    if (P.gain) v[j] = i * kVec + j < K ? __fmul_rn(v[j], P.gain[i * kVec + j]) : 0.f;
-                }
-            }
-        };
-        auto max_of = [&](const float (&v)[kVec]) {
-#pragma unroll
-            for (int j = 0; j < kVec; ++j) top = max(top, __float_as_uint(v[j]) & 0x7fffffffu);
-        };
 #pragma unroll
         for (int c = 0; c < kKeep; ++c) {
             const int i = threadIdx.x + c * step;
-            if (i < parts) value_at(i, keep[c]);
+            if (i < vecs) value_at(i, keep[c]);
             else
 #pragma unroll
                 for (int j = 0; j < kVec; ++j) keep[c][j] = 0.f;
         }
         if constexpr (PRO == kProNorm) {
             float sum = 0.f;
-#pragma unroll
-            for (int c = 0; c < kKeep; ++c)
-#pragma unroll
-                for (int j = 0; j < kVec; ++j) sum = fmaf(keep[c][j], keep[c][j], sum);
-            for (int i = threadIdx.x + kKeep * step; i < parts; i += step) {
-                float v[kVec];
-                value_at(i, v);
+            auto add_vec = [&](const float (&v)[kVec]) {
 #pragma unroll
                 for (int j = 0; j < kVec; ++j) sum = fmaf(v[j], v[j], sum);
+            };
+#pragma unroll
+            for (int c = 0; c < kKeep; ++c) add_vec(keep[c]);
+            for (int i = threadIdx.x + kKeep * step; i < vecs; i += step) {
+                float v[kVec];
+                value_at(i, v);
+                add_vec(v);
             }
+            for (int k = vecs * kVec + threadIdx.x; k < K; k += step) sum = fmaf(single(k), single(k), sum);
             rms = __fdiv_rn(1.f, __fsqrt_rn(__fadd_rn(__fdiv_rn(block_sum(sum, part_sum), static_cast<float>(K)), P.eps)));
 #pragma unroll
-            for (int c = 0; c < kKeep; ++c) {
-                const int i = threadIdx.x + c * step;
-                if (i < parts) scaled(i, keep[c]);
-            }
+            for (int c = 0; c < kKeep; ++c)
+                if (threadIdx.x + c * step < vecs) scaled_vec(threadIdx.x + c * step, keep[c]);
         }
 #pragma unroll
-        for (int c = 0; c < kKeep; ++c) max_of(keep[c]);
-        for (int i = threadIdx.x + kKeep * step; i < parts; i += step) {
+        for (int c = 0; c < kKeep; ++c) top = max_vec(top, keep[c]);
+        for (int i = threadIdx.x + kKeep * step; i < vecs; i += step) {
             float v[kVec];
             value_at(i, v);
-            scaled(i, v);
-            max_of(v);
-        }
-        set_scale();
-#pragma unroll
-        for (int c = 0; c < kKeep; ++c) {
-            const int i = threadIdx.x + c * step;
-            if (i < parts) store(i, keep[c]);
-        }
-        for (int i = threadIdx.x + kKeep * step; i < parts; i += step) {
-            float v[kVec];
-            value_at(i, v);
-            scaled(i, v);
-            store(i, v);
+            scaled_vec(i, v);
+            top = max_vec(top, v);
         }
     }
+    for (int k = vecs * kVec + threadIdx.x; k < K; k += step) top = max(top, bits(scaled(k, single(k))));
+    top = block_max(top, part_max);
+
+    // ---- the scale
+    const float a = __uint_as_float(top);
+    const bool bad = top >= 0x7f800000u;  // NaN or infinity
+    Scale c;
+    c.s = bad ? __uint_as_float(0x7fc00000u) : __fdiv_rn(a, 127.f);
+    if (threadIdx.x == 0) P.scale[r] = c.s;
+    if (bad || a < 0x1p-100f) {
+        for (int k = threadIdx.x; k < K; k += step) q[k] = bad ? 0 : quantize_tiny(scaled(k, single(k)), c.s);
+        return;
+    }
+    const float inv = __fdiv_rn(1.f, c.s);
+    c.lo = inv * (1.f - 0x1p-21f), c.hi = inv * (1.f + 0x1p-21f);
+
+    // ---- rounding
+#pragma unroll
+    for (int n = 0; n < kKeep; ++n) {
+        const int i = threadIdx.x + n * step;
+        if (i < vecs) {
+            if constexpr (PRO == kProNone) {
+                float v[kVec];
+                unpack<T>(raw[n], v);
+                store(i, v, c);
+            } else {
+                store(i, keep[n], c);
+            }
+        }
+    }
+    for (int i = threadIdx.x + kKeep * step; i < vecs; i += step) {
+        float v[kVec];
+        value_at(i, v);
+        scaled_vec(i, v);
+        store(i, v, c);
+    }
+    for (int k = vecs * kVec + threadIdx.x; k < K; k += step) q[k] = quantize1(scaled(k, single(k)), c);
 }
 
 template <typename T, bool VEC>
@@ -352,13 +383,14 @@ int launch_quantize_i8(const QuantizeI8& o, cudaStream_t stream) {
     const int size = o.x_type == kTypeF32 ? 4 : 2;
     uintptr_t bits = reinterpret_cast<uintptr_t>(o.x) | static_cast<uintptr_t>(o.x_stride * size);
     if (o.up) bits |= reinterpret_cast<uintptr_t>(o.up) | static_cast<uintptr_t>(o.up_stride * size);
-    const bool vec = (bits & 15) == 0;
+    const bool vec = (bits & 15) == 0 && ((reinterpret_cast<uintptr_t>(o.q) | static_cast<uintptr_t>(o.q_stride)) & 7) == 0;
     void (*kernel)(QuantizeI8) = nullptr;
     if (o.x_type == kTypeF32) kernel = vec ? pick<float, true>(o.kind) : pick<float, false>(o.kind);
     else if (o.x_type == kTypeF16) kernel = vec ? pick<__half, true>(o.kind) : pick<__half, false>(o.kind);
     else kernel = vec ? pick<__nv_bfloat16, true>(o.kind) : pick<__nv_bfloat16, false>(o.kind);
-    const int parts = (o.K + kVec - 1) / kVec;
-    const int want = o.N <= kFewRows ? parts : (parts + kKeep - 1) / kKeep;
+    const int parts = std::max(1, o.K / kVec);
+    const int keep = keep_vecs(size, o.kind);
+    const int want = o.N <= kFewRows ? parts : (parts + keep - 1) / keep;
     const int threads = std::min(kMaxThreads, (want + 31) / 32 * 32);
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(o.N);

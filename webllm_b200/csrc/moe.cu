@@ -30,9 +30,10 @@ __device__ __forceinline__ float to_f32(T v) {
 // One warp per token, E / 32 logits a lane in registers. A logit's key is its
 // bits in an unsigned order (0 for NaN and -inf, which are never chosen); each
 // of the k steps is one warp-wide maximum of the keys and one minimum of the
-// expert numbers that hold it, so ties go to the lowest expert. Bound: launch
-// latency for few tokens, the k dependent reductions for many (the logits are
-// read once: 4 E bytes a token).
+// expert numbers that hold it, so ties go to the lowest expert. The weights
+// are computed once, lane j the j-th's. Bound: launch latency for few tokens,
+// the k dependent reductions for many (the logits are read once: 4 E bytes a
+// token).
 constexpr int kRouteWarps = 4;
 
 template <typename T, int LANE>  // LANE: logits a lane holds, E <= 32 LANE
@@ -42,39 +43,22 @@ __global__ void __launch_bounds__(32 * kRouteWarps) route_kernel(const MoeRoute 
     const int64_t t = static_cast<int64_t>(blockIdx.x) * kRouteWarps + (threadIdx.x >> 5);
     if (t >= P.T) return;
     const T* row = static_cast<const T*>(P.logits) + t * P.stride;
+    const float none = __uint_as_float(0xff800000u);
     float l[LANE];
     uint32_t key[LANE];
 #pragma unroll
     for (int i = 0; i < LANE; ++i) {
         const int e = lane + 32 * i;
-        l[i] = e < P.E ? to_f32(row[e]) : __uint_as_float(0xff800000u);
+        l[i] = e < P.E ? to_f32(row[e]) : none;
     }
-    float top = __uint_as_float(0xff800000u);
 #pragma unroll
     for (int i = 0; i < LANE; ++i) {
         const uint32_t b = __float_as_uint(l[i] + 0.f);  // -0 and +0 are one value
-        const bool masked = !(l[i] > __uint_as_float(0xff800000u));
-        key[i] = masked ? 0u : ((b & 0x80000000u) ? ~b : (b | 0x80000000u));
-        if (!masked) top = fmaxf(top, l[i]);
-    }
-#pragma unroll
-    for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-    // exp(l - top); a logit of +inf counts as 1 and every finite one as 0 then
-    auto weight = [&](float v) {
-        if (P.score == kMoeSigmoid) return 1.f / (1.f + expf(-v));
-        return v == top ? 1.f : expf(v - top);
-    };
-    float all = 0.f;
-    if (P.score == kMoeSoftmax && !P.normalize) {
-#pragma unroll
-        for (int i = 0; i < LANE; ++i)
-            if (key[i]) all += weight(l[i]);
-#pragma unroll
-        for (int o = 16; o; o >>= 1) all += __shfl_xor_sync(0xffffffffu, all, o);
+        key[i] = !(l[i] > none) ? 0u : ((b & 0x80000000u) ? ~b : (b | 0x80000000u));
     }
     // lane j keeps the j-th choice
     int mine = -1;
-    float w = 0.f;
+    uint32_t mine_key = 0, first = 0;
     for (int j = 0; j < P.k; ++j) {
         uint32_t best = 0;
         int at = 0;
@@ -89,20 +73,30 @@ __global__ void __launch_bounds__(32 * kRouteWarps) route_kernel(const MoeRoute 
             for (int i = 0; i < LANE; ++i)
                 if (i == (e >> 5)) key[i] = 0;
         }
-        if (lane == j) {
-            mine = e;
-            const uint32_t b = (most & 0x80000000u) ? (most & 0x7fffffffu) : ~most;
-            w = weight(__uint_as_float(b));
-        }
+        if (lane == j) mine = e, mine_key = most;
+        if (j == 0) first = most;
     }
-    float sum = all;
-    if (P.normalize) {
-        sum = w;
+    auto value = [](uint32_t k) { return __uint_as_float((k & 0x80000000u) ? (k & 0x7fffffffu) : ~k); };
+    const float top = value(first);
+    // exp(l - top); a logit of +inf counts as 1 and every finite one as 0 then
+    auto weight = [&](float v) {
+        if (P.score == kMoeSigmoid) return 1.f / (1.f + expf(-v));
+        return v == top ? 1.f : expf(v - top);
+    };
+    float w = mine >= 0 ? weight(value(mine_key)) : 0.f;
+    if (P.normalize || P.score == kMoeSoftmax) {
+        float sum = w;
+        if (!P.normalize) {
+            sum = 0.f;
+#pragma unroll
+            for (int i = 0; i < LANE; ++i)
+                if (l[i] > none) sum += weight(l[i]);
+        }
 #pragma unroll
         for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+        w = sum > 0.f ? w / sum : 0.f;
     }
     if (lane < P.k) {
-        if (P.normalize || P.score == kMoeSoftmax) w = sum > 0.f ? w / sum : 0.f;
         P.ids[t * P.k + lane] = mine;
         P.weights[t * P.k + lane] = w * P.scale;
     }
@@ -110,73 +104,157 @@ __global__ void __launch_bounds__(32 * kRouteWarps) route_kernel(const MoeRoute 
 
 // ---------------------------------------------------------------- plan
 //
-// Slots in a stable order of their expert, without atomics: CTA e counts the
-// ids below e (its base) and places the slots of expert e behind it, in rising
-// order; CTA E does so for the slots without an expert (an id outside 0..E-1).
-// Every CTA reads all ids twice (from L2): 8 T k bytes, some microseconds up
-// to 65,536 slots, and no step waits on another CTA.
-constexpr int kPlanThreads = 512;
-constexpr int kPlanIds = 8;  // consecutive ids of a thread and step
+// Slots in a stable order of their key, the expert (E for an id outside
+// 0..E-1), without atomics and without workspace: one cluster of up to 8 CTAs,
+// each warp with a run of consecutive slots. Every warp counts its run's keys
+// (lanes with equal keys find each other with a ballot for each bit), the counts
+// of the warps before it, the CTAs before its own (distributed shared memory) and the
+// smaller keys give each key's first place, and a second walk over the run
+// places the slots. Bound: latency (8 T k bytes are moved, the ids twice from
+// L2); a CTA per expert that read all ids took 26 us for 65,536 slots and 128
+// experts.
+constexpr int kPlanWarps = 32;
+constexpr int kPlanCtas = 16;  // at most
 
-template <bool VEC>
-__device__ __forceinline__ void load_ids(const int32_t* ids, int64_t i, int64_t n, int E, int (&v)[kPlanIds]) {
-    if (VEC && i + kPlanIds <= n) {
-        const int4 a = *reinterpret_cast<const int4*>(ids + i), b = *reinterpret_cast<const int4*>(ids + i + 4);
-        v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
-    } else {
-#pragma unroll
-        for (int j = 0; j < kPlanIds; ++j) v[j] = i + j < n ? ids[i + j] : 0x7fffffff;
+constexpr int kPlanBatch = 8;   // ids a lane fetches at once
+
+__device__ __forceinline__ int plan_key(const int32_t* ids, int64_t i, int64_t end, int E) {
+    if (i >= end) return E + 1;  // no slot
+    const int id = ids[i];
+    return id < 0 || id >= E ? E : id;
+}
+// The lanes that hold the same key (of `bits` bits).
+__device__ __forceinline__ uint32_t same_key(int key, int bits) {
+    uint32_t same = 0xffffffffu;
+    for (int b = 0; b < bits; ++b) {
+        const bool set = (key >> b) & 1;
+        const uint32_t lanes = __ballot_sync(0xffffffffu, set);
+        same &= set ? lanes : ~lanes;
     }
-#pragma unroll
-    for (int j = 0; j < kPlanIds; ++j) {
-        if (i + j >= n) v[j] = E + 1;  // no slot
-        else if (v[j] < 0 || v[j] >= E) v[j] = E;
-    }
+    return same;
 }
 
-template <bool VEC>
-__global__ void __launch_bounds__(kPlanThreads) plan_kernel(const int32_t* ids, int64_t n, int E, int32_t* offsets,
-                                                            int32_t* order) {
-    __shared__ int part[2][kPlanThreads / 32];
+__global__ void __launch_bounds__(32 * kPlanWarps) plan_kernel(const int32_t* ids, int64_t n, int E, int32_t* offsets,
+                                                               int32_t* order) {
+    extern __shared__ int32_t plan_smem[];
+    const int keys = E + 1, warps = blockDim.x >> 5, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int ctas = static_cast<int>(gridDim.x), cta = static_cast<int>(blockIdx.x);
+    int32_t* count = plan_smem;               // [warps][keys], then each warp's next place among the CTA's
+    int32_t* total = count + warps * keys;    // [keys] of this CTA
+    int32_t* first = total + keys;            // [keys] where this CTA's slots of a key begin
+    __shared__ int32_t part[kPlanWarps];
+    for (int i = threadIdx.x; i < warps * keys; i += blockDim.x) count[i] = 0;
     pdl_begin();
-    const int e = blockIdx.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int warps = blockDim.x >> 5;
-    const int64_t step = static_cast<int64_t>(blockDim.x) * kPlanIds;
-    int below = 0;
-    for (int64_t i = static_cast<int64_t>(threadIdx.x) * kPlanIds; i < n; i += step) {
-        int v[kPlanIds];
-        load_ids<VEC>(ids, i, n, E, v);
-#pragma unroll
-        for (int j = 0; j < kPlanIds; ++j) below += v[j] < e;
-    }
-    below = __reduce_add_sync(0xffffffffu, below);
-    if (lane == 0) part[0][warp] = below;
+    const int bits = 32 - __clz(keys);  // of E + 1, the largest key
+    const int64_t all_warps = static_cast<int64_t>(ctas) * warps;
+    const int64_t run = (n + 32 * all_warps - 1) / (32 * all_warps) * 32;
+    const int64_t begin = (static_cast<int64_t>(cta) * warps + warp) * run, end = min(begin + run, n);
     __syncthreads();
-    int base = __reduce_add_sync(0xffffffffu, lane < warps ? part[0][lane] : 0);
-    if (threadIdx.x == 0) offsets[e] = base;
-    int flip = 1;
-    for (int64_t at = 0; at < n; at += step, flip ^= 1) {
-        const int64_t i = at + static_cast<int64_t>(threadIdx.x) * kPlanIds;
-        int v[kPlanIds];
-        load_ids<VEC>(ids, i, n, E, v);
-        int own = 0;
+    int32_t* own = count + warp * keys;
+    // every batch's ids are fetched together; a run of one batch keeps them for the second walk
+    int key[kPlanBatch];
+    auto fetch = [&](int64_t at) {
 #pragma unroll
-        for (int j = 0; j < kPlanIds; ++j) own += v[j] == e;
-        int before = own;  // inclusive sum over the warp
+        for (int j = 0; j < kPlanBatch; ++j) key[j] = plan_key(ids, at + 32 * j + lane, end, E);
+    };
+    for (int64_t at = begin; at < end; at += 32 * kPlanBatch) {
+        fetch(at);
+#pragma unroll
+        for (int j = 0; j < kPlanBatch; ++j) {
+            if (at + 32 * j >= end) break;
+            if (key[j] <= E) atomicAdd(&own[key[j]], 1);  // a count does not depend on the order
+        }
+    }
+    __syncthreads();
+    // counts of a key: exclusive over the warps (a lane each), and the CTA's total
+    if (warps <= 4) {  // few warps: a thread for each key
+        for (int e = threadIdx.x; e < keys; e += blockDim.x) {
+            int c[4], sum = 0;
+#pragma unroll
+            for (int w = 0; w < 4; ++w) c[w] = count[w * keys + e];
+#pragma unroll
+            for (int w = 0; w < 4; ++w) {
+                count[w * keys + e] = sum;
+                sum += c[w];
+            }
+            total[e] = sum;
+        }
+    } else
+    for (int e = warp; e < keys; e += warps) {
+        const int c = lane < warps ? count[lane * keys + e] : 0;
+        int sum = c;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
-            const int u = __shfl_up_sync(0xffffffffu, before, o);
-            if (lane >= o) before += u;
+            const int u = __shfl_up_sync(0xffffffffu, sum, o);
+            if (lane >= o) sum += u;
         }
-        if (lane == 31) part[flip][warp] = before;
-        __syncthreads();
-        const int w = lane < warps ? part[flip][lane] : 0;
-        int pos = base + before - own + __reduce_add_sync(0xffffffffu, lane < warp ? w : 0);
-        base += __reduce_add_sync(0xffffffffu, w);
-#pragma unroll
-        for (int j = 0; j < kPlanIds; ++j)
-            if (v[j] == e) order[pos++] = static_cast<int32_t>(i + j);
+        if (lane < warps) count[lane * keys + e] = sum - c;
+        if (lane == 31) total[e] = sum;
     }
+    __syncthreads();
+    if (ctas > 1) asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+    // a key's first place: smaller keys everywhere, then the CTAs before this one
+    int carry = 0;
+    for (int base = 0; base < keys; base += blockDim.x) {
+        const int e = base + threadIdx.x;
+        int everywhere = 0, before = 0;
+        if (e < keys) {
+            if (ctas == 1) {
+                everywhere = total[e];
+            } else {
+                const uint32_t at = static_cast<uint32_t>(__cvta_generic_to_shared(total + e));
+                int c[kPlanCtas];
+#pragma unroll
+                for (int r = 0; r < kPlanCtas; ++r) {
+                    uint32_t remote;
+                    c[r] = 0;
+                    if (r >= ctas) continue;
+                    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(at), "r"(r));
+                    asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(c[r]) : "r"(remote) : "memory");
+                }
+#pragma unroll
+                for (int r = 0; r < kPlanCtas; ++r) {
+                    everywhere += c[r];
+                    if (r < cta) before += c[r];
+                }
+            }
+        }
+        int sum = everywhere;  // inclusive over the warp
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int u = __shfl_up_sync(0xffffffffu, sum, o);
+            if (lane >= o) sum += u;
+        }
+        if (base) __syncthreads();  // part of the step before has been read
+        if (lane == 31) part[warp] = sum;
+        __syncthreads();
+        const int p = lane < warps ? part[lane] : 0;
+        const int smaller = carry + sum - everywhere + __reduce_add_sync(0xffffffffu, lane < warp ? p : 0);
+        carry += __reduce_add_sync(0xffffffffu, p);
+        if (e < keys) {
+            if (cta == 0) offsets[e] = smaller;
+            first[e] = smaller + before;
+        }
+    }
+    // no CTA ends while another reads its totals; what was read needs no order
+    if (ctas > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
+    __syncthreads();
+    for (int64_t at = begin; at < end; at += 32 * kPlanBatch) {
+        if (run > 32 * kPlanBatch) fetch(at);
+#pragma unroll
+        for (int j = 0; j < kPlanBatch; ++j) {
+            if (at + 32 * j >= end) break;
+            const uint32_t same = same_key(key[j], bits);
+            const int place = key[j] <= E ? first[key[j]] + own[key[j]] + __popc(same & ((1u << lane) - 1)) : 0;
+            __syncwarp();
+            if (key[j] <= E) {
+                order[place] = static_cast<int32_t>(at + 32 * j + lane);
+                if (lane == __ffs(same) - 1) own[key[j]] += __popc(same);
+            }
+            __syncwarp();
+        }
+    }
+    if (ctas > 1) asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
 }
 
 // ---------------------------------------------------------------- combine
@@ -297,9 +375,40 @@ int launch_moe_route(const MoeRoute& o, cudaStream_t stream) {
 }
 
 int launch_moe_plan(const int32_t* ids, int64_t slots, int E, int32_t* offsets, int32_t* order, cudaStream_t stream) {
-    const bool vec = (reinterpret_cast<uintptr_t>(ids) & 15) == 0;
-    const int threads = static_cast<int>(std::min<int64_t>(kPlanThreads, (std::max<int64_t>(slots, 1) + kPlanIds * 32 - 1) / (kPlanIds * 32) * 32));
-    return launch(vec ? plan_kernel<true> : plan_kernel<false>, dim3(E + 1), threads, stream, ids, slots, E, offsets, order);
+    // 64 slots a warp before there is another warp (four at least, for the walks
+    // over the keys), all warps of a CTA before another CTA
+    const int64_t want = std::max<int64_t>(4, (slots + 63) / 64);
+    const int warps = static_cast<int>(std::min<int64_t>(kPlanWarps, want));
+    const int ctas = static_cast<int>(std::min<int64_t>(kPlanCtas, (want + kPlanWarps - 1) / kPlanWarps));
+    const int smem = (warps + 2) * (E + 1) * 4;
+    if (smem > 48 * 1024 || ctas > 8) {
+        static bool configured[kMaxDevices] = {};  // the attribute is per device
+        int dev = 0;
+        if (const cudaError_t e = cudaGetDevice(&dev); e != cudaSuccess) return -static_cast<int>(e);
+        if (dev < 0 || dev >= kMaxDevices) return -static_cast<int>(cudaErrorInvalidDevice);
+        if (!configured[dev]) {
+            cudaError_t e = cudaFuncSetAttribute(plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                                 (kPlanWarps + 2) * (kMaxExperts + 1) * 4);
+            if (e == cudaSuccess) e = cudaFuncSetAttribute(plan_kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+            if (e != cudaSuccess) return -static_cast<int>(e);
+            configured[dev] = true;
+        }
+    }
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(ctas);
+    cfg.blockDim = dim3(32 * warps);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = static_cast<unsigned>(ctas);
+    attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 2;
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, plan_kernel, ids, slots, E, offsets, order);
+    return e == cudaSuccess ? 1 : -static_cast<int>(e);
 }
 
 int launch_moe_combine(const MoeCombine& o, cudaStream_t stream) {

@@ -450,21 +450,20 @@ __global__ void __launch_bounds__(GROUPED ? kThreads + kLoaders : kThreads, 1) i
     Walk<GROUPED, MODE> walk{P, cum, begin};
 
     if (warp == 0) {
-        // ---------------- copies ----------------
-        Ring ring{stages};
-        int filled = 0;  // stages filled so far, up to the ring's size
-        bool ok = true;
-        for (int i = item0; i < items && ok; i += item_step) {
-            const Item it = walk.at(i);
-            const int m0 = it.m0 + (PAIR ? kTileM * rank : 0);
-            const int cols = (it.rows + 31) & ~31, n0 = it.first + (PAIR ? rank * (cols / 2) : 0);
-            for (int c = c0; c < c1; ++c) {
-                const int s = ring.s;
-                ok = filled < stages || mbar_wait(&empty[s], ring.parity ^ 1, 1u, poisoned);
-                ok = __all_sync(0xffffffffu, ok);
-                if (!ok) break;
-                const uint32_t a = smem_u32(smem + s * stage_bytes);
-                if (elect_one()) {
+        if (elect_one()) {
+            // ---------------- copies ----------------
+            Ring ring{stages};
+            int filled = 0;  // stages filled so far, up to the ring's size
+            bool ok = true;
+            for (int i = item0; i < items && ok; i += item_step) {
+                const Item it = walk.at(i);
+                const int m0 = it.m0 + (PAIR ? kTileM * rank : 0);
+                const int cols = (it.rows + 31) & ~31, n0 = it.first + (PAIR ? rank * (cols / 2) : 0);
+                for (int c = c0; c < c1; ++c) {
+                    const int s = ring.s;
+                    ok = filled < stages || mbar_wait(&empty[s], ring.parity ^ 1, 1u, poisoned);
+                    if (!ok) break;
+                    const uint32_t a = smem_u32(smem + s * stage_bytes);
                     const uint32_t b = a + kSub * kABytes;
                     if constexpr (PAIR) {
                         if (rank == 0) mbar_expect_tx(&full[s], 2 * (GROUPED ? kSub * kABytes : stage_bytes));
@@ -482,22 +481,21 @@ __global__ void __launch_bounds__(GROUPED ? kThreads + kLoaders : kThreads, 1) i
                             if constexpr (!GROUPED) tma_2d(b + h * b_bytes, &P.xmap, k, n0, &full[s]);
                         }
                     }
+                    if (filled < stages) ++filled;
+                    ring.next();
                 }
-                __syncwarp();
-                if (filled < stages) ++filled;
-                ring.next();
             }
-        }
-        if (*poisoned && rank == 0) {  // the copies in flight land before the CTA ends
-            for (int p = 0; p < filled; ++p) {
-                ring.s = ring.s ? ring.s - 1 : (ring.parity ^= 1, stages - 1);
-                mbar_drain(&full[ring.s], ring.parity);
+            if (*poisoned && (!PAIR || rank == 0)) {  // the copies in flight land before the CTA ends
+                for (int p = 0; p < filled; ++p) {
+                    ring.s = ring.s ? ring.s - 1 : (ring.parity ^= 1, stages - 1);
+                    mbar_drain(&full[ring.s], ring.parity);
+                }
             }
         }
     } else if (warp == 1) {
         Ring ring{stages};
         bool ok = true;
-        if (!PAIR || rank == 0) {
+        if ((!PAIR || rank == 0) && elect_one()) {
             // ---------------- MMAs ----------------
             uint32_t t = 0;
             uint64_t* last = nullptr;  // the barrier of the last commit, and its parity
@@ -507,7 +505,6 @@ __global__ void __launch_bounds__(GROUPED ? kThreads + kLoaders : kThreads, 1) i
                 const uint32_t idesc = PAIR ? i8_idesc(2 * kTileM, (it.rows + 31) & ~31) : i8_idesc(kTileM, (it.rows + 15) & ~15);
                 const uint32_t buf = t & 1, d = tmem + buf * P.tile_n;
                 ok = t < 2 || mbar_wait(&acc_free[buf], ((t >> 1) - 1) & 1, 2u, poisoned);
-                ok = __all_sync(0xffffffffu, ok);
                 if (!ok) break;
                 tc_fence_after();
                 for (int c = c0; c < c1; ++c) {
@@ -517,37 +514,30 @@ __global__ void __launch_bounds__(GROUPED ? kThreads + kLoaders : kThreads, 1) i
                         ok = ok && mbar_wait(&b_full[s], ring.parity, 4u, poisoned);
                         fence_async();  // the gathered tokens were written by the generic proxy
                     }
-                    ok = __all_sync(0xffffffffu, ok);
                     if (!ok) break;
                     tc_fence_after();
                     const uint32_t a = smem_u32(smem + s * stage_bytes);
-                    if (elect_one()) {
 #pragma unroll
-                        for (int h = 0; h < kSub; ++h) {
-                            const uint64_t ad = umma_desc(a + h * kABytes), bd = umma_desc(a + kSub * kABytes + h * b_bytes);
+                    for (int h = 0; h < kSub; ++h) {
+                        const uint64_t ad = umma_desc(a + h * kABytes), bd = umma_desc(a + kSub * kABytes + h * b_bytes);
 #pragma unroll
-                            for (int j = 0; j < kChunk / 32; ++j) {
-                                const uint32_t more = c > c0 || h > 0 || j > 0;
-                                if constexpr (PAIR) umma_i8_pair(d, ad + 2 * j, bd + 2 * j, idesc, more);
-                                else umma_i8(d, ad + 2 * j, bd + 2 * j, idesc, more);
-                            }
+                        for (int j = 0; j < kChunk / 32; ++j) {
+                            const uint32_t more = c > c0 || h > 0 || j > 0;
+                            if constexpr (PAIR) umma_i8_pair(d, ad + 2 * j, bd + 2 * j, idesc, more);
+                            else umma_i8(d, ad + 2 * j, bd + 2 * j, idesc, more);
                         }
-                        if constexpr (PAIR) umma_commit_pair(&empty[s]);
-                        else umma_commit(&empty[s]);
                     }
-                    __syncwarp();
+                    if constexpr (PAIR) umma_commit_pair(&empty[s]);
+                    else umma_commit(&empty[s]);
                     last = &empty[s], last_parity = ring.parity;
                     ring.next();
                 }
-                if (elect_one()) {
-                    if constexpr (PAIR) umma_commit_pair(&acc_full[buf]);
-                    else umma_commit(&acc_full[buf]);
-                }
-                __syncwarp();
+                if constexpr (PAIR) umma_commit_pair(&acc_full[buf]);
+                else umma_commit(&acc_full[buf]);
             }
             // MMAs still in flight (only after a time-out) end before the TMEM is freed
             if (*poisoned && last) mbar_drain(last, last_parity);
-        } else if constexpr (GROUPED) {
+        } else if (GROUPED && PAIR && rank) {
             // ---------------- this CTA's tokens are ready, told to the pair's first ----------------
             for (int i = item0; i < items && ok; i += item_step)
                 for (int c = c0; c < c1; ++c) {
