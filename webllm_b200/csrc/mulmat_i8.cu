@@ -14,13 +14,13 @@
 //  - warp 0 (TMA): per 128-byte chunk of K one box of 128 weight rows, and of
 //    dense tokens one box of the tile's rows, into a ring of stages (K-major,
 //    128-byte swizzle).
-//  - warps 6..9 (grouped only): an expert's tokens are gathered through the
+//  - warps 10..17 (grouped only): an expert's tokens are gathered through the
 //    sorted slots with 16-byte cp.async, straight into the swizzled layout, so
 //    no sorted copy of the activations is ever written. (TMA's gather of four
 //    rows a copy took 18 cycles a row: 1045 us against GATHER_US for 4096 tokens
 //    in 8 of 128 experts, 1536 -> 4096.)
 //  - warp 1 (MMA): one thread issues the 4 K=32 MMAs of a chunk.
-//  - warps 2..5 (epilogue): TMEM -> scales -> y, while the next tile's MMAs
+//  - warps 2..9 (epilogue): TMEM -> scales -> y, while the next tile's MMAs
 //    fill the other accumulator. An item's rows and scales are fetched ahead of
 //    the wait for its accumulator.
 //
@@ -64,11 +64,12 @@ constexpr int kMaxShortN = 128; // of a pair's with two chunks a stage
 constexpr int kMaxSingleN = 64; // of a single CTA's or a split one
 constexpr int kChunk = 128;    // bytes of K of a swizzled row
 constexpr int kABytes = kTileM * kChunk;
-constexpr int kThreads = 192;       // copies, MMAs, four epilogue warps
-constexpr int kLoaders = 128;       // threads that gather tokens
+constexpr int kEpiWarps = 8;        // two for each quarter of the TMEM lanes
+constexpr int kThreads = 64 + 32 * kEpiWarps;  // copies, MMAs, epilogue
+constexpr int kLoaders = 128;       // threads that gather a stage's tokens; there are two such groups
 constexpr int kMaxStages = 12;
 constexpr int kPrefetch = 16;       // chunks of weights brought into L2 ahead of the launch's dependency
-constexpr int kSmemBytes = 213 * 1024;  // dynamic, beside up to 13 KB of tables and barriers
+constexpr int kSmemBytes = 208 * 1024;  // dynamic, beside up to 17 KB of tables and barriers
 constexpr uint32_t kSpinLimit = 1u << 26;
 
 struct I8Args {
@@ -155,10 +156,6 @@ __device__ __forceinline__ void tma_3d_pair(uint32_t dst, const CUtensorMap* tm,
 // 16 bytes to shared memory, zeros where bytes is 0.
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, uint32_t bytes) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
-}
-// Arrives on bar when this thread's cp.async so far have landed.
-__device__ __forceinline__ void cp_async_arrive(uint64_t* bar) {
-    asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
 }
 // Arrives on the barrier at bar's place in CTA `rank` of the cluster. What it
 // orders is not memory that the other CTA's threads read, but the tensor pipe's
@@ -263,13 +260,51 @@ __device__ __forceinline__ int4 ld_cluster4(uint32_t local, uint32_t rank) {
     return v;
 }
 
-// y in its type: the two scales in f32, then one rounding.
+// Two f32 in a register pair, and their packed arithmetic.
+__device__ __forceinline__ uint64_t pack2(uint32_t a, uint32_t b) { return static_cast<uint64_t>(b) << 32 | a; }
+__device__ __forceinline__ uint64_t pack2(float a, float b) { return pack2(__float_as_uint(a), __float_as_uint(b)); }
+__device__ __forceinline__ float low(uint64_t v) { return __uint_as_float(static_cast<uint32_t>(v)); }
+__device__ __forceinline__ float high(uint64_t v) { return __uint_as_float(static_cast<uint32_t>(v >> 32)); }
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+    uint64_t d;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+    return d;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+    uint64_t d;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+    return d;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+    return d;
+}
+
+// y in its type: the sum in f32, times the two scales in f32, then one rounding.
 __device__ __forceinline__ float scaled(int32_t acc, float s, float t) { return __fmul_rn(__fmul_rn(__int2float_rn(acc), s), t); }
+// The same of two sums, without the conversion pipe (8 clocks a warp and sum,
+// more than an item's MMAs leave at K = 1536): the halves hi, lo of a sum are
+// exact as floats (as_float(2^23's bits + lo) - 2^23), and hi * 65536 + lo is one
+// FMA, so the conversion is rounded once, as __int2float_rn's.
+__device__ __forceinline__ uint64_t scaled2(int32_t a, int32_t b, uint64_t s, uint64_t t) {
+    const uint64_t hi = add2(pack2(static_cast<uint32_t>(0x4B400000 + (a >> 16)), static_cast<uint32_t>(0x4B400000 + (b >> 16))),
+                             pack2(-12582912.f, -12582912.f));
+    const uint64_t lo = add2(pack2(0x4B000000u | (a & 0xffff), 0x4B000000u | (b & 0xffff)), pack2(-8388608.f, -8388608.f));
+    return mul2(mul2(fma2(hi, pack2(65536.f, 65536.f), lo), s), t);
+}
 __device__ __forceinline__ void put(float* p, float v) { *p = v; }
 __device__ __forceinline__ void put(__half* p, float v) { *p = __float2half_rn(v); }
 __device__ __forceinline__ void put(__nv_bfloat16* p, float v) { *p = __float2bfloat16_rn(v); }
-__device__ __forceinline__ void store_y(const MulMatI8& o, int64_t row, int m, float v) {
-    const int64_t at = row * o.y_stride + m;
+__device__ __forceinline__ uint32_t half_pair(const __half*, uint64_t v) {
+    const __half2 h = __floats2half2_rn(low(v), high(v));
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+__device__ __forceinline__ uint32_t half_pair(const __nv_bfloat16*, uint64_t v) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(low(v), high(v));
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+__device__ __forceinline__ void store_y(const MulMatI8& o, int64_t at, float v) {
     if (o.y_type == kTypeF32) put(static_cast<float*>(o.y) + at, v);
     else if (o.y_type == kTypeF16) put(static_cast<__half*>(o.y) + at, v);
     else put(static_cast<__nv_bfloat16*>(o.y) + at, v);
@@ -316,43 +351,56 @@ struct Walk {
     }
 };
 
-// The rows of an accumulator that this warp holds, into y: column n of the tile
-// is token row[n] with scale s[n].
+// Every other 16 columns of an accumulator, of the 32 lanes (channels) that this
+// warp holds, into y: column n of the tile is the row at[n] (elements from y's
+// start) with scale s[n].
 template <typename T>
-__device__ __forceinline__ void store_tile(const MulMatI8& o, uint32_t taddr, int rows, int m, float tm, const int32_t* row,
+__device__ __forceinline__ void store_tile(const MulMatI8& o, uint32_t taddr, int first, int rows, int m, float tm, const int64_t* at,
                                            const float* s) {
     T* y = static_cast<T*>(o.y) + m;
-    const bool live = m < o.M;
-    int n = 0;
-    if (__all_sync(0xffffffffu, live)) {  // no branch between the 16 stores
-        for (; n + 16 <= rows; n += 16) {
-            int32_t acc[16];
-            tmem_ld16(taddr + n, acc);
-#pragma unroll
-            for (int j = 0; j < 16; ++j) put(y + row[n + j] * o.y_stride, scaled(acc[j], s[n + j], tm));
-        }
-    }
-    for (; n < rows; n += 16) {
+    const int lane = threadIdx.x & 31;
+    const bool live = m < o.M, whole = __all_sync(0xffffffffu, live);
+    // 16-bit values of two neighbouring channels go out as one word: the lanes of
+    // a pair exchange one of their two columns
+    const bool words = sizeof(T) == 2 && (reinterpret_cast<uintptr_t>(o.y) & 3) == 0 && (o.y_stride & 1) == 0;
+    const uint64_t t2 = pack2(tm, tm);
+    for (int n = first; n < rows; n += 32) {
         int32_t acc[16];
         tmem_ld16(taddr + n, acc);
+        if (whole && n + 16 <= rows && (sizeof(T) == 4 || words)) {  // no branch between the stores
 #pragma unroll
-        for (int j = 0; j < 16; ++j)
-            if (n + j < rows && live) put(y + row[n + j] * o.y_stride, scaled(acc[j], s[n + j], tm));
+            for (int j = 0; j < 16; j += 2) {
+                const uint64_t v = scaled2(acc[j], acc[j + 1], *reinterpret_cast<const uint64_t*>(s + n + j), t2);
+                if constexpr (sizeof(T) == 4) {
+                    put(y + at[n + j], low(v));
+                    put(y + at[n + j + 1], high(v));
+                } else {
+                    const uint32_t own = half_pair(y, v), other = __shfl_xor_sync(0xffffffffu, own, 1);
+                    // even lanes: column j of channels m, m + 1; odd: column j + 1 of m - 1, m
+                    const uint32_t w = lane & 1 ? __byte_perm(other, own, 0x7632) : __byte_perm(own, other, 0x5410);
+                    *reinterpret_cast<uint32_t*>(y - (lane & 1) + at[n + j + (lane & 1)]) = w;
+                }
+            }
+        } else {
+#pragma unroll
+            for (int j = 0; j < 16; ++j)
+                if (n + j < rows && live) put(y + at[n + j], scaled(acc[j], s[n + j], tm));
+        }
     }
 }
 
 template <bool GROUPED, int MODE>
-__global__ void __launch_bounds__(GROUPED ? kThreads + kLoaders : kThreads, 1) i8_kernel(const __grid_constant__ I8Args P) {
+__global__ void __launch_bounds__(GROUPED ? kThreads + 2 * kLoaders : kThreads, 1) i8_kernel(const __grid_constant__ I8Args P) {
     constexpr bool SPLIT = MODE == kSplit, PAIR = is_pair(MODE);
     constexpr int kTokens = MODE == kPair ? kMaxTileN : (PAIR ? kMaxShortN : kMaxSingleN);
     extern __shared__ __align__(1024) uint8_t smem_raw[];
-    __shared__ uint64_t full[kMaxStages], b_full[kMaxStages], empty[kMaxStages], acc_full[2], acc_free[2];
+    __shared__ uint64_t full[kMaxStages], empty[kMaxStages], acc_full[2], acc_free[2];
     __shared__ uint32_t tmem_slot;
     __shared__ int poison;
     __shared__ int32_t cum[GROUPED ? kMaxExperts + 1 : 1], begin[GROUPED ? kMaxExperts + 1 : 1];
-    __shared__ int32_t warp_sum[10];
-    __shared__ int32_t out_row[2][kTokens];
-    __shared__ float out_scale[2][kTokens];
+    __shared__ int32_t warp_sum[(kThreads + 2 * kLoaders) / 32];
+    __shared__ int64_t out_at[2][kTokens];  // where a tile's rows begin in y
+    __shared__ __align__(8) float out_scale[2][kTokens];
     // 1024-byte alignment for the swizzled tiles
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     volatile int* poisoned = &poison;
@@ -370,13 +418,12 @@ __global__ void __launch_bounds__(GROUPED ? kThreads + kLoaders : kThreads, 1) i
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < stages; ++s) {
-            mbar_init(&full[s], PAIR && GROUPED ? 2 : 1);
-            mbar_init(&b_full[s], kLoaders);
+            mbar_init(&full[s], 1 + (GROUPED ? (PAIR ? 2 : 1) * kLoaders / 32 : 0));
             mbar_init(&empty[s], 1);
         }
         for (int b = 0; b < 2; ++b) {
             mbar_init(&acc_full[b], 1);
-            mbar_init(&acc_free[b], PAIR ? 8 : 4);
+            mbar_init(&acc_free[b], (PAIR ? 2 : 1) * kEpiWarps);
         }
         poison = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -428,7 +475,7 @@ __global__ void __launch_bounds__(GROUPED ? kThreads + kLoaders : kThreads, 1) i
             if (lane == 31) warp_sum[warp] = sum;
             __syncthreads();
             int before = carry;
-            for (int w = 0; w < (kThreads + kLoaders) / 32; ++w) {
+            for (int w = 0; w < (kThreads + 2 * kLoaders) / 32; ++w) {
                 if (w < warp) before += warp_sum[w];
                 carry += warp_sum[w];
             }
@@ -510,10 +557,6 @@ __global__ void __launch_bounds__(GROUPED ? kThreads + kLoaders : kThreads, 1) i
                 for (int c = c0; c < c1; ++c) {
                     const int s = ring.s;
                     ok = mbar_wait(&full[s], ring.parity, 4u, poisoned);
-                    if constexpr (GROUPED) {
-                        ok = ok && mbar_wait(&b_full[s], ring.parity, 4u, poisoned);
-                        fence_async();  // the gathered tokens were written by the generic proxy
-                    }
                     if (!ok) break;
                     tc_fence_after();
                     const uint32_t a = smem_u32(smem + s * stage_bytes);
@@ -537,35 +580,26 @@ __global__ void __launch_bounds__(GROUPED ? kThreads + kLoaders : kThreads, 1) i
             }
             // MMAs still in flight (only after a time-out) end before the TMEM is freed
             if (*poisoned && last) mbar_drain(last, last_parity);
-        } else if (GROUPED && PAIR && rank) {
-            // ---------------- this CTA's tokens are ready, told to the pair's first ----------------
-            for (int i = item0; i < items && ok; i += item_step)
-                for (int c = c0; c < c1; ++c) {
-                    ok = mbar_wait(&b_full[ring.s], ring.parity, 4u, poisoned);
-                    if (!ok) break;
-                    fence_async();
-                    if (lane == 0) mbar_arrive_at(&full[ring.s], 0);
-                    ring.next();
-                }
         }
-    } else if (warp < 6) {
+    } else if (warp < 2 + kEpiWarps) {
         // ---------------- epilogue ----------------
-        const int quad = warp & 3;  // the TMEM lanes this warp may read
+        const int quad = warp & 3;                // the TMEM lanes this warp may read
+        const int n0 = (warp - 2) / 4 % 2 * 16;   // it takes every other 16 columns, from here on
         uint32_t t = 0;
         for (int i = item0; i < items; i += item_step, ++t) {
             const Item it = walk.at(i);
             const uint32_t buf = t & 1;
             const int m = it.m0 + (PAIR ? kTileM * rank : 0) + 32 * quad + lane;
             const float tm = m < P.o.M ? P.o.w_scale[static_cast<int64_t>(it.e) * P.o.M + m] : 0.f;
-            for (int n = threadIdx.x - 64; n < it.rows; n += 128) {
+            for (int n = threadIdx.x - 64; n < it.rows; n += 32 * kEpiWarps) {
                 int row = it.first + n;
                 if constexpr (GROUPED) row = P.o.order[row];
-                out_row[buf][n] = row;
+                out_at[buf][n] = row * P.o.y_stride;
                 out_scale[buf][n] = P.o.q_scale[!GROUPED || P.o.per_slot ? row : row / P.o.k];
             }
-            asm volatile("bar.sync 1, 128;" ::: "memory");  // the epilogue warps
-            // after a time-out the items are still walked (the four warps meet at the
-            // barrier above), without their stores
+            asm volatile("bar.sync 1, %0;" ::"n"(32 * kEpiWarps) : "memory");  // the epilogue warps
+            // after a time-out the items are still walked (the epilogue's warps meet at
+            // the barrier above), without their stores
             const bool ok = mbar_wait(&acc_full[buf], (t >> 1) & 1, 2u, poisoned);
             tc_fence_after();
             const uint32_t d = tmem + buf * P.tile_n + (static_cast<uint32_t>(32 * quad) << 16);
@@ -573,18 +607,18 @@ __global__ void __launch_bounds__(GROUPED ? kThreads + kLoaders : kThreads, 1) i
             } else if constexpr (SPLIT) {
                 // the stages are free by now: all copies have landed and all MMAs have read them
                 int32_t* part = reinterpret_cast<int32_t*>(smem) + 32 * quad + lane;
-                for (int n = 0; n < it.rows; n += 16) {
+                for (int n = n0; n < it.rows; n += 32) {
                     int32_t acc[16];
                     tmem_ld16(d + n, acc);
 #pragma unroll
                     for (int j = 0; j < 16; ++j) part[(n + j) * kTileM] = acc[j];
                 }
             } else if (P.o.y_type == kTypeF32) {
-                store_tile<float>(P.o, d, it.rows, m, tm, out_row[buf], out_scale[buf]);
+                store_tile<float>(P.o, d, n0, it.rows, m, tm, out_at[buf], out_scale[buf]);
             } else if (P.o.y_type == kTypeF16) {
-                store_tile<__half>(P.o, d, it.rows, m, tm, out_row[buf], out_scale[buf]);
+                store_tile<__half>(P.o, d, n0, it.rows, m, tm, out_at[buf], out_scale[buf]);
             } else {
-                store_tile<__nv_bfloat16>(P.o, d, it.rows, m, tm, out_row[buf], out_scale[buf]);
+                store_tile<__nv_bfloat16>(P.o, d, n0, it.rows, m, tm, out_at[buf], out_scale[buf]);
             }
             tc_fence_before();
             __syncwarp();
@@ -595,50 +629,74 @@ __global__ void __launch_bounds__(GROUPED ? kThreads + kLoaders : kThreads, 1) i
         }
     } else if constexpr (GROUPED) {
         // ---------------- gathered tokens ----------------
-        // thread x takes 16-byte piece x % 8 of rows x / 8, x / 8 + 16, ..
-        const int x = threadIdx.x - kThreads, piece = x & 7, r0 = x >> 3;
+        // Two groups of threads take the stages in turn, so that one's address
+        // and barrier work overlaps the other's. Of a stage, thread x of a group
+        // takes 16-byte piece x % 8 of rows x / 8, x / 8 + 16, ..
+        const int x = (threadIdx.x - kThreads) % kLoaders, piece = x & 7, r0 = x >> 3;
+        const int mine = (threadIdx.x - kThreads) / kLoaders;
         constexpr int kRows = (PAIR ? kTokens / 2 : kTokens) / 16;
+        auto cols_of = [&](const Item& it) { return PAIR ? ((it.rows + 31) & ~31) / 2 : (it.rows + 15) & ~15; };  // of this CTA
+        int slot[kRows];
+        auto fetch = [&](const Item& it) {
+            const int cols = cols_of(it), skip = PAIR ? static_cast<int>(rank) * cols : 0;
+#pragma unroll
+            for (int r = 0; r < kRows; ++r)  // what is behind the last row reads that row again
+                if (r * 16 < cols) slot[r] = P.o.order[it.first + min(skip + r0 + 16 * r, it.rows - 1)];
+        };
+        Item it{};
+        if (item0 < items) fetch(it = walk.at(item0));
+        // A stage is told to the MMA thread (of the pair's first CTA) when the
+        // group's next one has been issued and this one has landed: one arrival a
+        // warp, and the fence for the tensor pipe's proxy by the threads that
+        // wrote. (An arrival of every thread, triggered by its copies, took 128
+        // arrivals a stage on one barrier, and a pair's second CTA a warp that
+        // passed them on: 900 clocks a chunk, whatever the copies.)
+        auto tell = [&](int s) {
+            fence_async();
+            __syncwarp();
+            if (lane == 0) {
+                if constexpr (PAIR) mbar_arrive_at(&full[s], 0);
+                else mbar_arrive(&full[s]);
+            }
+        };
         Ring ring{stages};
-        int filled = 0;
+        int q = 0, untold = -1;  // stages so far; the group's stage that has not been told
         bool ok = true;
         for (int i = item0; i < items && ok; i += item_step) {
-            const Item it = walk.at(i);
-            const int cols = PAIR ? ((it.rows + 31) & ~31) / 2 : (it.rows + 15) & ~15;  // of this CTA, a multiple of 16
-            const int skip = PAIR ? static_cast<int>(rank) * cols : 0;
-            int from[kRows];
+            const int cols = cols_of(it);
+            const int8_t* row[kRows];
 #pragma unroll
-            for (int r = 0; r < kRows; ++r) {
-                if (r * 16 >= cols) break;
-                // what is behind the last row reads that row again
-                const int slot = P.o.order[it.first + min(skip + r0 + 16 * r, it.rows - 1)];
-                from[r] = P.o.per_slot ? slot : slot / P.o.k;
-            }
-            for (int c = c0; c < c1; ++c) {
+            for (int r = 0; r < kRows; ++r)
+                row[r] = P.o.q + (r * 16 < cols ? static_cast<int64_t>(P.o.per_slot ? slot[r] : slot[r] / P.o.k) * P.o.q_stride : 0);
+            if (i + item_step < items) fetch(it = walk.at(i + item_step));  // the next item's, while this one's are copied
+            for (int c = c0; c < c1; ++c, ++q, ring.next()) {
+                if ((q & 1) != mine) continue;
                 const int s = ring.s;
-                if (filled < stages) ++filled;
-                else if (!mbar_wait(&empty[s], ring.parity ^ 1, 1u, poisoned)) {
-                    ok = false;
-                    break;
-                }
+                ok = q < stages || mbar_wait(&empty[s], ring.parity ^ 1, 1u, poisoned);
+                ok = __all_sync(0xffffffffu, ok);
+                if (!ok) break;
                 // piece p of row r lies at r * 128 + (p ^ (r % 8)) * 16; bytes behind K, where
                 // the weights are zeros, may hold anything, but nothing is read behind the row
 #pragma unroll
                 for (int h = 0; h < kSub; ++h) {
                     const int k = (c * kSub + h) * kChunk + piece * 16;
-                    const int8_t* src = P.o.q + (k < P.o.K ? k : 0);
                     const uint32_t bytes = k < P.o.K ? 16 : 0;
+                    const int at = k < P.o.K ? k : 0;
                     const uint32_t dst = smem_u32(smem + s * stage_bytes) + kSub * kABytes + h * b_bytes + r0 * kChunk + ((piece ^ (r0 & 7)) << 4);
 #pragma unroll
-                    for (int r = 0; r < kRows; ++r) {
-                        if (r * 16 >= cols) break;
-                        cp_async16(dst + r * 16 * kChunk, src + from[r] * P.o.q_stride, bytes);
-                    }
+                    for (int r = 0; r < kRows; ++r)
+                        if (r * 16 < cols) cp_async16(dst + r * 16 * kChunk, row[r] + at, bytes);
                 }
-                cp_async_arrive(&b_full[s]);
-                ring.next();
+                asm volatile("cp.async.commit_group;" ::: "memory");
+                if (untold >= 0) {
+                    asm volatile("cp.async.wait_group 1;" ::: "memory");
+                    tell(untold);
+                }
+                untold = s;
             }
         }
         asm volatile("cp.async.wait_all;" ::: "memory");
+        if (untold >= 0) tell(untold);
     }
     if constexpr (SPLIT) {
         // one item per cluster, so that the sum over the splits comes after all roles
@@ -662,7 +720,7 @@ __global__ void __launch_bounds__(GROUPED ? kThreads + kLoaders : kThreads, 1) i
 #pragma unroll
                 for (int j = 0; j < 4; ++j)
                     if (m + j < P.o.M)
-                        store_y(P.o, out_row[0][n], m + j,
+                        store_y(P.o, out_at[0][n] + m + j,
                                 scaled(acc[j], out_scale[0][n], P.o.w_scale[static_cast<int64_t>(it.e) * P.o.M + m + j]));
             }
         }
@@ -671,7 +729,7 @@ __global__ void __launch_bounds__(GROUPED ? kThreads + kLoaders : kThreads, 1) i
         // slots without an expert come last in the order: their rows are zero
         for (int64_t p = P.o.offsets[P.o.E] + blockIdx.x; p < P.o.slots; p += gridDim.x) {
             const int64_t row = P.o.order[p];
-            for (int m = threadIdx.x; m < P.o.M; m += blockDim.x) store_y(P.o, row, m, 0.f);
+            for (int m = threadIdx.x; m < P.o.M; m += blockDim.x) store_y(P.o, row * P.o.y_stride + m, 0.f);
         }
     }
     __syncwarp();
@@ -704,7 +762,7 @@ __global__ void __launch_bounds__(256) i8_general_kernel(const MulMatI8 o) {
             row = o.order[p];
             from = o.per_slot ? row : row / o.k;
             if (p >= o.offsets[o.E]) {
-                if (lane == 0) store_y(o, row, m, 0.f);
+                if (lane == 0) store_y(o, row * o.y_stride + m, 0.f);
                 continue;
             }
             int hi = o.E - 1;  // the last expert whose first slot is at or before p
@@ -719,7 +777,7 @@ __global__ void __launch_bounds__(256) i8_general_kernel(const MulMatI8 o) {
         int acc = 0;
         for (int k = lane; k < o.K; k += 32) acc += static_cast<int>(w[k]) * q[k];
         acc = __reduce_add_sync(0xffffffffu, acc);
-        if (lane == 0) store_y(o, row, m, scaled(acc, o.q_scale[from], o.w_scale[static_cast<int64_t>(e) * o.M + m]));
+        if (lane == 0) store_y(o, row * o.y_stride + m, scaled(acc, o.q_scale[from], o.w_scale[static_cast<int64_t>(e) * o.M + m]));
     }
 }
 
@@ -834,7 +892,7 @@ int launch(const MulMatI8& o, cudaStream_t stream, int num_sms) {
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(static_cast<unsigned>(
         plan.mode == kSplit ? plan.items * group : std::min<int64_t>(plan.items, num_sms / group) * group));
-    cfg.blockDim = dim3(GROUPED ? kThreads + kLoaders : kThreads);
+    cfg.blockDim = dim3(GROUPED ? kThreads + 2 * kLoaders : kThreads);
     cfg.dynamicSmemBytes = 1024 + P.stages * stage_bytes;
     cfg.stream = stream;
     cudaLaunchAttribute attr[2];
