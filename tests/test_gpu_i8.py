@@ -15,6 +15,9 @@ Tolerances, with u = eps / 2 of a type (half a step, relative to the value):
 """
 from __future__ import annotations
 
+import os
+import subprocess
+import sys
 import zlib
 
 import numpy as np
@@ -242,6 +245,22 @@ def test_product(rt, torch, t, M, K, N):
     close(torch, run_product(torch, w, ws, q, qs, M, K, N, t), ref_product(torch, w, ws, q, qs, K))
 
 
+def test_product_many_shapes(rt, torch):
+    """Sizes drawn over the whole range, so that every mode, token tile and split of the kernel's plan comes up, with
+    whole and ragged tiles, even and odd output strides."""
+    rng = np.random.default_rng(5)
+    for i in range(60):
+        M, K, N = (int(np.exp(rng.uniform(np.log(lo), np.log(hi)))) for lo, hi in ((1, 3000), (1, 6000), (1, 1500)))
+        g = gen_of(torch, "many", i)
+        w, ws = weights8(torch, g, M, K)
+        q, qs = weights8(torch, g, N, K)
+        t = ("f32", "f16", "bf16")[i % 3]
+        wide = torch.full((N, M + i % 4), 5.0, dtype=types(torch)[t][0], device="cuda")
+        run_product(torch, w, ws, q, qs, M, K, N, t, y=wide[:, :M])
+        close(torch, wide[:, :M], ref_product(torch, w, ws, q, qs, K))
+        assert (wide[:, M:] == 5).all(), (M, K, N)
+
+
 @pytest.mark.parametrize("M,K,N", [(200, 131071, 3), (130, 131071, 70)])
 def test_product_largest_sums(rt, torch, M, K, N):
     """Every product at its largest: 131071 * 128 * 128 is the largest sum below 2^31."""
@@ -396,7 +415,7 @@ def plan_of(torch, ids, E):
 
 
 @pytest.mark.parametrize("T,k,E", [(1, 1, 1), (1, 8, 64), (3, 2, 5), (513, 3, 7), (511, 8, 128), (4096, 4, 60), (8192, 8, 128),
-                                   (2049, 2, 1024), (40000, 2, 3)])
+                                   (2049, 2, 1024), (40000, 2, 3), (8192, 8, 1024), (200000, 8, 300)])
 def test_plan(rt, torch, T, k, E):
     g = gen_of(torch, "plan", T, k, E)
     ids = torch.randint(-2, E + 2, (T, k), dtype=torch.int32, device="cuda", generator=g)  # some outside 0..E-1
@@ -465,6 +484,27 @@ def test_grouped(rt, torch, per_slot, how, T, k, E, M, K):
     ref = ref_grouped(torch, w, ws, q, qs, per_slot, ids, K)
     for t in ("f32", "bf16"):
         close(torch, run_grouped(torch, w, ws, q, qs, per_slot, offsets, order, M, K, E, T, k, t), ref)
+
+
+def test_grouped_many_shapes(rt, torch):
+    """Sizes and routings drawn over the whole range, skewed ones among them."""
+    rng = np.random.default_rng(6)
+    for i in range(40):
+        T, M, K = (int(np.exp(rng.uniform(np.log(lo), np.log(hi)))) for lo, hi in ((1, 2000), (1, 1200), (1, 2000)))
+        E = int(rng.integers(1, 40))
+        k = int(rng.integers(1, min(E, 8) + 1))
+        g = gen_of(torch, "grouped many", i)
+        w, ws = weights8(torch, g, E * M, K)
+        w, ws = w.view(E, M, -1), ws.view(E, M)
+        per_slot = bool(i & 1)
+        q, qs = weights8(torch, g, T * k if per_slot else T, K)
+        like = torch.randn(E, device="cuda", generator=g) * (i % 5)  # how much some experts are liked
+        ids = (torch.randn(T, E, device="cuda", generator=g) + like).topk(k, 1).indices.to(torch.int32)
+        ids[torch.rand(T, k, device="cuda", generator=g) < 0.1 * (i % 3)] = -1
+        offsets, order = plan_of(torch, ids, E)
+        t = ("f32", "f16", "bf16")[i % 3]
+        y = run_grouped(torch, w, ws, q, qs, per_slot, offsets, order, M, K, E, T, k, t)
+        close(torch, y, ref_grouped(torch, w, ws, q, qs, per_slot, ids, K))
 
 
 @pytest.mark.parametrize("pitch,gap", [(0, 0), (5, 0), (16, 64), (16, 8)])
@@ -589,6 +629,67 @@ def test_captured_layers_share_nothing(rt, torch):
             moe_layer(torch, *a, fresh)
             torch.cuda.synchronize()
             assert torch.equal(fresh["y"], b["y"])
+
+
+CAPTURED_FIRST = """
+import torch
+from webllm_b200 import jsep
+jsep.install_jsep_callbacks(0)
+T, K, E, k, M = 70, 256, 8, 2, 384
+x = torch.randn(T, K, device="cuda")
+w, t = torch.randint(-127, 128, (E, M, K), dtype=torch.int8, device="cuda"), torch.rand(E, M, device="cuda")
+n = lambda *s, t=torch.float32: torch.zeros(*s, dtype=t, device="cuda")
+ids, wt, of, od = n(T, k, t=torch.int32), n(T, k), n(E + 1, t=torch.int32), n(T * k, t=torch.int32)
+q, s, y, z, d = n(T, K, t=torch.int8), n(T), n(T * k, M), n(T, M), n(T, M)
+l = torch.randn(T, E, device="cuda")
+def calls():
+    st = torch.cuda.current_stream().cuda_stream or jsep.STREAM_LEGACY
+    jsep.moe_route(l.data_ptr(), E, T, E, k, jsep.MOE_SOFTMAX, True, 1.0, ids.data_ptr(), wt.data_ptr(), stream=st)
+    jsep.moe_plan(ids.data_ptr(), T, k, E, of.data_ptr(), od.data_ptr(), stream=st)
+    jsep.quantize_i8(0, x.data_ptr(), K, T, K, q.data_ptr(), K, s.data_ptr(), stream=st)
+    jsep.mul_mat_id_i8(w.data_ptr(), K, M * K, t.data_ptr(), q.data_ptr(), K, s.data_ptr(), False, of.data_ptr(), od.data_ptr(), 0,
+                       y.data_ptr(), M, M, K, E, T, k, stream=st)
+    jsep.moe_combine(0, y.data_ptr(), M, wt.data_ptr(), 0, z.data_ptr(), M, T, k, M, stream=st)
+    jsep.mul_mat_i8(w.data_ptr(), K, t.data_ptr(), q.data_ptr(), K, s.data_ptr(), 0, d.data_ptr(), M, M, K, T, stream=st)
+torch.cuda.synchronize()
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g):
+    calls()
+g.replay()
+torch.cuda.synchronize()
+z1, d1 = z.clone(), d.clone()
+z.zero_(), d.zero_()
+calls()
+torch.cuda.synchronize()
+assert z1.abs().sum() > 0 and torch.equal(z, z1) and torch.equal(d, d1)
+print("captured first")
+"""
+
+
+def test_first_calls_may_be_captured():
+    """In a new process the first calls of all are made while a stream is being captured."""
+    r = subprocess.run([sys.executable, "-c", CAPTURED_FIRST], cwd=os.path.dirname(os.path.dirname(os.path.abspath(__file__))),
+                       capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and "captured first" in r.stdout, r.stdout[-1500:] + r.stderr[-1500:]
+
+
+def test_many_streams_at_once(rt, torch):
+    """Different products at the same time on four streams, pairs and splits among them: each what it is alone."""
+    shapes = [(512, 1024, 300), (3000, 512, 1), (256, 4096, 40), (1024, 2048, 130)]
+    work = []
+    for M, K, N in shapes:
+        g = gen_of(torch, "streams", M)
+        w, ws = weights8(torch, g, M, K)
+        q, qs = weights8(torch, g, N, K)
+        work.append((M, K, N, w, ws, q, qs, run_product(torch, w, ws, q, qs, M, K, N), torch.zeros(N, M, device="cuda"), torch.cuda.Stream()))
+    torch.cuda.synchronize()
+    for _ in range(25):
+        for M, K, N, w, ws, q, qs, _, y, st in work:
+            jsep.mul_mat_i8(w.data_ptr(), w.stride(0), ws.data_ptr(), q.data_ptr(), q.stride(0), qs.data_ptr(), 0, y.data_ptr(), M, M, K, N,
+                            stream=st.cuda_stream)
+    torch.cuda.synchronize()
+    for *_, alone, y, _ in work:
+        assert torch.equal(alone, y)
 
 
 def test_library_stream_and_its_graphs(rt, torch):

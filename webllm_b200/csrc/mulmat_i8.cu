@@ -49,6 +49,7 @@
 #include <stdint.h>
 
 #include <algorithm>
+#include <cmath>
 
 #include "wllm_internal.h"
 
@@ -813,35 +814,85 @@ int launch_general(const MulMatI8& o, cudaStream_t stream, int num_sms) {
     return e == cudaSuccess ? 1 : -static_cast<int>(e);
 }
 
-// The mode, the token tile and how many items there are at most.
+// The mode, the token tile, the split of K and how many items there are at most.
 struct Plan {
     Mode mode;
     int tile_n, splits;
     int64_t items;
 };
 
+// Clocks that a launch is expected to take, from what its parts were measured
+// to: a stage costs its MMAs, its bytes from L2 (57 a clock and SM, 45 over all
+// SMs), or the 380 clocks of its waits and issue; an item some 600 more, where K
+// is split 4000 and 50 a token (the cluster's start and barrier, the sum of the
+// tiles). Clusters of 2, 4 and 8 leave SMs of a GPC unused. What HBM adds is the
+// same for all plans. Grouped, the items are the expected ones of an even
+// routing. (Against the best of all plans, forced one by one, over 20 shapes
+// from 1 x 4096 x 4096 to 2000 tokens in 4 of 256 experts: within 15% but for one
+// at 19%.)
+template <bool GROUPED>
+double clocks(const MulMatI8& o, const Plan& p, int num_sms, double used) {
+    const bool pair = is_pair(p.mode);
+    const int sub = chunks_of_stage(p.mode), step = pair ? 32 : 16, tile_m = pair ? 2 * kTileM : kTileM;
+    const double tiles_m = (o.M + tile_m - 1) / tile_m;
+    double items, cols = p.tile_n;
+    if (GROUPED) {
+        const double mean = o.slots / used;
+        const double tiles = mean <= p.tile_n / 2 ? 1.0 : mean / p.tile_n + 0.5;  // of an expert, ragged groups among them
+        items = used * tiles * tiles_m;
+        cols = std::min<double>(p.tile_n, std::ceil(mean / tiles / step) * step);
+    } else {
+        items = static_cast<double>((o.N + p.tile_n - 1) / p.tile_n) * tiles_m;
+    }
+    const int lost = p.splits == 8 ? 4 : (p.splits == 4 ? 3 : (p.splits == 2 ? 2 : 0));
+    const double units = std::max(1, num_sms / (pair ? 2 : p.splits) - lost);
+    const double waves = GROUPED ? std::max(1.0, items / units + 0.5) : std::ceil(items / units);
+    const int chunks = (o.K + sub * kChunk - 1) / (sub * kChunk);
+    const double mma = 4.0 * sub * std::max(36.0, cols / 2), bytes = sub * (kABytes + (pair ? cols / 2 : cols) * kChunk);
+    const double stage = std::max(380.0, std::max(mma, bytes / 57));
+    const double own = waves * ((chunks + p.splits - 1) / p.splits * stage + (p.splits > 1 ? 4000.0 + 50 * cols : 600.0));
+    return std::max(own, items * chunks * bytes * (pair ? 2 : 1) / (45.0 * num_sms));
+}
+
 template <bool GROUPED>
 Plan plan(const MulMatI8& o, int num_sms) {
-    Plan p{kSingle, 16, 1, 0};
-    // tokens that a tile should hold: all of them, or an expert's mean share,
-    // doubled (groups are ragged)
-    const int64_t want = GROUPED ? std::min<int64_t>((2 * o.slots + o.E - 1) / o.E, o.slots) : o.N;
-    if (want > kMaxSingleN && o.M > kTileM) p.mode = want <= kMaxShortN ? kPairShort : kPair;
-    const bool pair = is_pair(p.mode);
-    const int most = pair ? kMaxTileN : kMaxSingleN, step = pair ? 32 : 16;
-    const int64_t tiles = (want + most - 1) / most;
-    p.tile_n = static_cast<int>(((want + tiles - 1) / tiles + step - 1) / step * step);
-    const int m = pair ? 2 * kTileM : kTileM;
-    const int64_t tiles_m = (o.M + m - 1) / m;
-    // at most one started tile more than the whole ones of each expert
-    const int64_t tiles_n = GROUPED ? std::min<int64_t>(o.slots, o.slots / p.tile_n + o.E) : (o.N + p.tile_n - 1) / p.tile_n;
-    p.items = tiles_n * tiles_m;
+    Plan best{};
+    double best_clocks = 0;
+    // experts that an even routing reaches
+    const double used = GROUPED ? std::max(1.0, o.E * (1.0 - std::exp(-static_cast<double>(o.slots) / o.E))) : 1.0;
+    auto consider = [&](Mode mode, int tile_n, int splits) {
+        const Plan p{mode, tile_n, splits, 0};
+        const double c = clocks<GROUPED>(o, p, num_sms, used);
+        if (best.tile_n == 0 || c < best_clocks) best = p, best_clocks = c;
+    };
+    // token tiles worth a look: of a dense product those that cover N in equal
+    // parts, as few as the mode allows or up to seven more; of groups all sizes
+    // up to the slots
+    auto sizes = [&](int most, int step, auto&& use) {
+        if (GROUPED) {
+            for (int n = step; n <= most; n += n < 64 ? step : 64) {
+                use(n);
+                if (n >= o.slots) break;
+            }
+        } else {
+            const int least = (o.N + most - 1) / most;
+            for (int tiles = least; tiles < least + 8; ++tiles) {
+                const int n = ((o.N + tiles - 1) / tiles + step - 1) / step * step;
+                use(n);
+                if (n == step) break;
+            }
+        }
+    };
     const int chunks = (o.K + 2 * kChunk - 1) / (2 * kChunk);
-    if (p.mode == kSingle)
-        while (p.splits < 8 && p.items * p.splits * 2 <= num_sms && chunks >= p.splits * 2) p.splits *= 2;
-    if (p.splits > 1) p.mode = kSplit;
-    if (pair && p.tile_n <= kMaxShortN) p.mode = kPairShort;
-    return p;
+    sizes(kMaxSingleN, 16, [&](int n) {
+        for (int s = 1; s <= 8 && s <= chunks; s *= 2) consider(s > 1 ? kSplit : kSingle, n, s);
+    });
+    if (o.M > kTileM) sizes(kMaxTileN, 32, [&](int n) { consider(n <= kMaxShortN ? kPairShort : kPair, n, 1); });
+    const int tile_m = is_pair(best.mode) ? 2 * kTileM : kTileM;
+    const int64_t tiles_m = (o.M + tile_m - 1) / tile_m;
+    // of groups at most one started tile more than the whole ones of each expert
+    best.items = tiles_m * (GROUPED ? std::min<int64_t>(o.slots, o.slots / best.tile_n + o.E) : (o.N + best.tile_n - 1) / best.tile_n);
+    return best;
 }
 
 template <bool GROUPED>
@@ -909,10 +960,21 @@ int launch(const MulMatI8& o, cudaStream_t stream, int num_sms) {
 
 }  // namespace
 
-int launch_mul_mat_i8(const MulMatI8& o, cudaStream_t stream, int num_sms) { return launch<false>(o, stream, num_sms); }
-int launch_mul_mat_id_i8(const MulMatI8& o, cudaStream_t stream, int num_sms) { return launch<true>(o, stream, num_sms); }
+// Whether there has been a launch whose waits could have given up: hosts that
+// use none of this pay nothing for it in wllm_sync.
+static bool g_i8_launched = false;
+
+int launch_mul_mat_i8(const MulMatI8& o, cudaStream_t stream, int num_sms) {
+    g_i8_launched = true;
+    return launch<false>(o, stream, num_sms);
+}
+int launch_mul_mat_id_i8(const MulMatI8& o, cudaStream_t stream, int num_sms) {
+    g_i8_launched = true;
+    return launch<true>(o, stream, num_sms);
+}
 
 unsigned read_and_clear_i8_error() {
+    if (!g_i8_launched) return 0;
     unsigned v = 0;
     if (cudaMemcpyFromSymbol(&v, g_i8_error, sizeof(v)) != cudaSuccess) return 0xFFFFFFFFu;
     if (v) {
