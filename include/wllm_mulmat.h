@@ -306,9 +306,11 @@ int32_t wllm_dequantize(int32_t type, const void* src, float* dst, int64_t n, vo
  * They run on the device of wllm_init whatever the calling thread's current
  * device is, use no library workspace, allocate nothing and never wait, so
  * calls on several streams are independent and each may be captured into a
- * graph. Inputs are not modified; an output may overlap no input of its call
- * (WLLM_STATUS_FAILED where the library can see it). Extents are not checked.
- * N = 0 tokens (rows) is allowed and does nothing. */
+ * graph, its first one too. Inputs are not modified; an output may overlap no
+ * input of its call (WLLM_STATUS_FAILED where the library can see it). Extents
+ * are not checked. N = 0 rows (tokens) is allowed and writes nothing (but
+ * wllm_moe_plan its offsets, all zero). Results do not depend on timing: no sum
+ * is taken in an order that varies. */
 
 /* N rows of K values to int8 with one scale each:
  *   a = max_k |v_k|, scale = a / 127 in f32, q_k = the integer nearest v_k / scale

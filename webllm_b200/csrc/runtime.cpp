@@ -1117,10 +1117,14 @@ private:
     cudaError_t err_ = cudaSuccess;
 };
 
-// Byte range of n rows of len elements, stride apart.
+// Byte range of n rows of len elements, stride apart (to the address space's
+// end where it is larger).
 ByteRange rows_range(const void* p, int64_t stride, int64_t n, int64_t len, int size) {
     const uintptr_t b = reinterpret_cast<uintptr_t>(p);
-    return {b, b + (p && n > 0 ? static_cast<uintptr_t>(size) * static_cast<uintptr_t>(stride * (n - 1) + len) : 0)};
+    if (!p || n <= 0) return {b, b};
+    const unsigned __int128 bytes =
+        (static_cast<unsigned __int128>(stride) * static_cast<unsigned __int128>(n - 1) + static_cast<unsigned __int128>(len)) * size;
+    return {b, bytes > UINTPTR_MAX - b ? UINTPTR_MAX : b + static_cast<uintptr_t>(bytes)};
 }
 
 bool aligned(const void* p, int size) { return (reinterpret_cast<uintptr_t>(p) & (size - 1)) == 0; }
