@@ -17,7 +17,10 @@
 // A row that holds a NaN or an infinity has no scale: s = NaN and q = 0, so
 // every product of it is NaN.
 //
-// Bound: HBM (one read of the row, K + 4 bytes written). One CTA per row; the
+// Bound: HBM (one read of the row, K + 4 bytes written): 8192 x 14336 bf16 in 54
+// us, 6.5 TB/s; 4096 x 14336 f32 in 43.5 us, 6.8 TB/s; silu(gate) * up of 32768
+// x 1536 bf16 in 55 us, 4.6 TB/s, there bound by its exponentials too. One CTA
+// per row; the
 // row's values stay in registers between the maximum and the rounding, so rows
 // up to 32 values a thread are read once; longer rows are read again (from L2)
 // in the second pass.
@@ -115,16 +118,44 @@ __device__ __forceinline__ uint32_t top_bits(uint32_t top) {
     return h << 16;
 }
 
+// Two f32 in a register pair, and their packed arithmetic.
+__device__ __forceinline__ uint64_t pack2(float a, float b) {
+    return static_cast<uint64_t>(__float_as_uint(b)) << 32 | __float_as_uint(a);
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+    return d;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+    uint64_t d;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+    return d;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+    uint64_t d;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+    return d;
+}
+__device__ __forceinline__ float low(uint64_t v) { return __uint_as_float(static_cast<uint32_t>(v)); }
+__device__ __forceinline__ float high(uint64_t v) { return __uint_as_float(static_cast<uint32_t>(v >> 32)); }
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ float rcp(float x) {
+    float y;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
 // silu(g) * u and gelu(g) * u, as wllm_mul_mat_glu_batch computes them: x / (1 +
 // e^-z) with the SFU's exponential and reciprocal. What they flush to zero (an
 // e^-z below 2^-126, a reciprocal of more than 2^126) is lost in the sum or the
 // product anyway.
-__device__ __forceinline__ float x_sigmoid(float x, float z) {
-    float e, r;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(z * -1.4426950408889634f));
-    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.f + e));
-    return x * r;
-}
+constexpr float kLog2e = 1.4426950408889634f;
+__device__ __forceinline__ float x_sigmoid(float x, float z) { return x * rcp(1.f + ex2(z * -kLog2e)); }
 __device__ __forceinline__ float glu(int kind, float g, float u) {
     if (kind == kProSwiglu) return __fmul_rn(x_sigmoid(g, g), u);
     float y;
@@ -138,6 +169,22 @@ __device__ __forceinline__ float glu(int kind, float g, float u) {
         y = __half2float(__float2half_rn(x_sigmoid(f, 2.f * s)));
     }
     return __fmul_rn(y, u);
+}
+
+// The same of a vector, silu two values an instruction.
+__device__ __forceinline__ void glu8(int kind, float (&v)[kVec], const float (&u)[kVec]) {
+    if (kind == kProSwiglu) {
+#pragma unroll
+        for (int j = 0; j < kVec; j += 2) {
+            const uint64_t g = pack2(v[j], v[j + 1]), z = mul2(g, pack2(-kLog2e, -kLog2e));
+            const uint64_t d = add2(pack2(ex2(low(z)), ex2(high(z))), pack2(1.f, 1.f));
+            const uint64_t y = mul2(mul2(g, pack2(rcp(low(d)), rcp(high(d)))), pack2(u[j], u[j + 1]));
+            v[j] = low(y), v[j + 1] = high(y);
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < kVec; ++j) v[j] = glu(kind, v[j], u[j]);
+    }
 }
 
 // Block-wide maximum (of bits) and sum; `part` holds one word per warp.
@@ -158,15 +205,6 @@ __device__ __forceinline__ float block_sum(float v, float* part) {
 #pragma unroll
     for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
     return v;
-}
-
-__device__ __forceinline__ uint64_t pack2(float a, float b) {
-    return static_cast<uint64_t>(__float_as_uint(b)) << 32 | __float_as_uint(a);
-}
-__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
-    uint64_t d;
-    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
-    return d;
 }
 
 constexpr float kMagic = 12582912.f;  // 1.5 * 2^23: a sum with it is rounded to the nearest integer (ties to even)
@@ -238,8 +276,7 @@ __global__ void __launch_bounds__(kMaxThreads, 2) quantize_i8_kernel(const Quant
         if constexpr (PRO == kProSwiglu) {
             float u[kVec];
             unpack<T>(b, u);
-#pragma unroll
-            for (int j = 0; j < kVec; ++j) v[j] = glu(P.kind, v[j], u[j]);
+            glu8(P.kind, v, u);
         }
     };
     auto value_at = [&](int i, float (&v)[kVec]) {
@@ -262,10 +299,11 @@ __global__ void __launch_bounds__(kMaxThreads, 2) quantize_i8_kernel(const Quant
         return PRO == kProSwiglu ? glu(P.kind, v, to_f32(up[k])) : v;
     };
     auto bits = [](float v) { return __float_as_uint(v) & 0x7fffffffu; };
-    auto max_vec = [&](uint32_t top, const float (&v)[kVec]) {
+    // a NaN stays in `most`, as one whose bits are above infinity's
+    auto max_vec = [&](float most, const float (&v)[kVec]) {
 #pragma unroll
-        for (int j = 0; j < kVec; ++j) top = max(top, bits(v[j]));
-        return top;
+        for (int j = 0; j < kVec; ++j) asm("max.NaN.f32 %0, %0, %1;" : "+f"(most) : "f"(fabsf(v[j])));
+        return most;
     };
     auto store = [&](int i, const float (&v)[kVec], const Scale& c) {
         const uint2 w = quantize8(v, c);
@@ -323,14 +361,16 @@ __global__ void __launch_bounds__(kMaxThreads, 2) quantize_i8_kernel(const Quant
             for (int c = 0; c < kKeep; ++c)
                 if (threadIdx.x + c * step < vecs) scaled_vec(threadIdx.x + c * step, keep[c]);
         }
+        float most = 0.f;
 #pragma unroll
-        for (int c = 0; c < kKeep; ++c) top = max_vec(top, keep[c]);
+        for (int c = 0; c < kKeep; ++c) most = max_vec(most, keep[c]);
         for (int i = threadIdx.x + kKeep * step; i < vecs; i += step) {
             float v[kVec];
             value_at(i, v);
             scaled_vec(i, v);
-            top = max_vec(top, v);
+            most = max_vec(most, v);
         }
+        top = bits(most);
     }
     for (int k = vecs * kVec + threadIdx.x; k < K; k += step) top = max(top, bits(scaled(k, single(k))));
     top = block_max(top, part_max);

@@ -33,7 +33,7 @@ __device__ __forceinline__ float to_f32(T v) {
 // expert numbers that hold it, so ties go to the lowest expert. The weights
 // are computed once, lane j the j-th's. Bound: launch latency for few tokens,
 // the k dependent reductions for many (the logits are read once: 4 E bytes a
-// token).
+// token): 8192 tokens, 8 of 128 experts, 8.6 us.
 constexpr int kRouteWarps = 4;
 
 template <typename T, int LANE>  // LANE: logits a lane holds, E <= 32 LANE
@@ -105,14 +105,14 @@ __global__ void __launch_bounds__(32 * kRouteWarps) route_kernel(const MoeRoute 
 // ---------------------------------------------------------------- plan
 //
 // Slots in a stable order of their key, the expert (E for an id outside
-// 0..E-1), without atomics and without workspace: one cluster of up to 8 CTAs,
-// each warp with a run of consecutive slots. Every warp counts its run's keys
-// (lanes with equal keys find each other with a ballot for each bit), the counts
-// of the warps before it, the CTAs before its own (distributed shared memory) and the
-// smaller keys give each key's first place, and a second walk over the run
-// places the slots. Bound: latency (8 T k bytes are moved, the ids twice from
-// L2); a CTA per expert that read all ids took 26 us for 65,536 slots and 128
-// experts.
+// 0..E-1), without global atomics and without workspace: one cluster of up to 16
+// CTAs, each warp with a run of consecutive slots. Every warp counts its run's
+// keys in shared memory; the counts of the warps before it, of the CTAs before
+// its own (distributed shared memory) and of the smaller keys give each key's
+// first place, and a second walk over the run places the slots, lanes with equal
+// keys in their order (they find each other with a ballot for each bit). Bound:
+// latency (8 T k bytes are moved): 10 us for 65,536 slots and 128 experts, 4 for
+// 8 slots; a CTA per expert that read all ids took 26, 8 CTAs 17.
 constexpr int kPlanWarps = 32;
 constexpr int kPlanCtas = 16;  // at most
 
@@ -261,7 +261,8 @@ __global__ void __launch_bounds__(32 * kPlanWarps) plan_kernel(const int32_t* id
 //
 // y[t][m] = sum_j weight[t][j] z[t k + j][m], in f32 and in the order of j (no
 // atomics, so the sum does not depend on timing). Bound: HBM or L2, one read of
-// the slots' rows; a thread takes 16 bytes of each.
+// the slots' rows; a thread takes 16 bytes of each: 4096 tokens, 8 f16 rows of
+// 4096, 44 us, 6.9 TB/s.
 template <typename T, int N>
 __device__ __forceinline__ void load_n(const T* p, float (&v)[N]) {
     if constexpr (N == 1) {

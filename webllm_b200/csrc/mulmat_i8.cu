@@ -17,28 +17,31 @@
 //  - warps 10..17 (grouped only): an expert's tokens are gathered through the
 //    sorted slots with 16-byte cp.async, straight into the swizzled layout, so
 //    no sorted copy of the activations is ever written. (TMA's gather of four
-//    rows a copy took 18 cycles a row: 1045 us against GATHER_US for 4096 tokens
-//    in 8 of 128 experts, 1536 -> 4096.)
+//    rows a copy is slower: 648 us against 399 for the step of 4096 tokens in 8
+//    of 128 experts, 1536 -> 4096, at the time that both were tried, and 80
+//    against 58 for 512 tokens in 8 of 64, 2048 -> 2048.)
 //  - warp 1 (MMA): one thread issues the 4 K=32 MMAs of a chunk.
 //  - warps 2..9 (epilogue): TMEM -> scales -> y, while the next tile's MMAs
 //    fill the other accumulator. An item's rows and scales are fetched ahead of
 //    the wait for its accumulator.
 //
 // CTAs are persistent over the items (expert, channel tile, token tile), in one
-// of three modes (plan() says which):
+// of these modes (plan() chooses by a model of their cost):
 //  - single: an item is 128 channels;
 //  - pair: two CTAs of a cluster share an item of 256 channels (cta_group::2):
 //    each loads its own 128 weight rows and half of the tokens, which both read,
 //    so a chunk of a 256-token tile takes 32 KB of an SM's L2 bandwidth instead
-//    of 48;
+//    of 48 (8192^3: 2960 TOP/s; a single CTA per item, 2430);
 //  - split: where the items are fewer than the SMs (single tokens, small
 //    batches), S = 2, 4 or 8 CTAs of a cluster share an item's K: each leaves
 //    its int32 tile in its own shared memory, and after a cluster barrier CTA r
 //    adds the S tiles of its share of the columns through distributed shared
 //    memory.
 //
-// Bounds: HBM (the weights, once) up to a few hundred tokens, the tensor pipe
-// above.
+// Bounds: HBM (the weights, once) up to a few hundred tokens (1 x 4096 -> 14336:
+// 13 us, of which some 4 are set-up, first bytes and the last tile), the tensor
+// pipe above (4096 x 14336 -> 4096: 160 us, 3.0 POP/s; in a long run the power
+// limit, 2.5 to 2.8).
 //
 // Every mbarrier wait is bounded: on time-out the CTA records an error code
 // (read by wllm_sync), stops issuing, waits for its copies and MMAs in flight
