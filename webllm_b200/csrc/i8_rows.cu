@@ -25,7 +25,9 @@
 // up to 32 values a thread are read once; longer rows are read again (from L2)
 // in the second pass.
 // Threads: rows that are few take one 8-value vector a thread (latency), many
-// rows as many as its registers keep (fewer barriers a byte).
+// rows as many as its registers keep (fewer barriers a byte), and many short rows
+// a warp each, eight a CTA (25,960 x 256, silu(gate) * up: 14 us against 29
+// with a CTA a row).
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <stdint.h>
@@ -43,6 +45,7 @@ constexpr int kVec = 8;    // values of a thread's vector
 // prologue) as f32.
 __host__ __device__ constexpr int keep_vecs(int size, int pro) { return size == 2 && pro == kProNone ? 8 : 4; }
 constexpr int kMaxThreads = 512;
+constexpr int kWarpRows = 8;   // rows of a CTA whose warps take one each
 constexpr int kFewRows = 512;  // at most this many rows: one vector a thread
 
 // A thread's vector of 8 values as it lies in memory.
@@ -70,24 +73,39 @@ __device__ __forceinline__ void unpack(const Raw<T>& r, float (&v)[kVec]) {
     }
 }
 
-// Values [8 i, 8 i + 8) of a row. VEC: the row starts on a 16-byte boundary.
+// Values [8 i, 8 i + 8) of a row. VEC: the row starts on a 16-byte boundary;
+// otherwise they are shifted out of the 16-byte words that they lie in (each of
+// which holds at least one of them, so no word that is read is wholly outside
+// the row). Every vector of a row is shifted alike.
 template <typename T, bool VEC>
 __device__ __forceinline__ Raw<T> load_vec(const T* row, int i) {
+    constexpr int kPieces = Raw<T>::kWords / 4;
     Raw<T> r;
+    const uintptr_t at = reinterpret_cast<uintptr_t>(row + static_cast<int64_t>(i) * kVec);
+    const uint4* p = reinterpret_cast<const uint4*>(at & ~static_cast<uintptr_t>(15));
+    const uint32_t off = VEC ? 0 : static_cast<uint32_t>(at & 15);
+    uint32_t w[4 * kPieces + 4];
+#pragma unroll
+    for (int h = 0; h < kPieces + (VEC ? 0 : 1); ++h) {
+        const uint4 a = h < kPieces || off ? p[h] : make_uint4(0, 0, 0, 0);
+        w[4 * h] = a.x, w[4 * h + 1] = a.y, w[4 * h + 2] = a.z, w[4 * h + 3] = a.w;
+    }
     if constexpr (VEC) {
-        const uint4* p = reinterpret_cast<const uint4*>(row + static_cast<int64_t>(i) * kVec);
 #pragma unroll
-        for (int h = 0; h < Raw<T>::kWords / 4; ++h) {
-            const uint4 a = p[h];
-            r.w[4 * h] = a.x, r.w[4 * h + 1] = a.y, r.w[4 * h + 2] = a.z, r.w[4 * h + 3] = a.w;
-        }
-    } else if constexpr (sizeof(T) == 4) {
-#pragma unroll
-        for (int j = 0; j < kVec; ++j) r.w[j] = reinterpret_cast<const uint32_t*>(row)[static_cast<int64_t>(i) * kVec + j];
+        for (int h = 0; h < Raw<T>::kWords; ++h) r.w[h] = w[h];
     } else {
-        const uint16_t* p = reinterpret_cast<const uint16_t*>(row) + static_cast<int64_t>(i) * kVec;
+        // by words, then by bytes
+        const uint32_t words = off >> 2, bits = (off & 3) * 8;
+        if (words & 2) {
 #pragma unroll
-        for (int h = 0; h < kVec / 2; ++h) r.w[h] = p[2 * h] | static_cast<uint32_t>(p[2 * h + 1]) << 16;
+            for (int h = 0; h + 2 < 4 * kPieces + 4; ++h) w[h] = w[h + 2];
+        }
+        if (words & 1) {
+#pragma unroll
+            for (int h = 0; h + 1 < 4 * kPieces + 4; ++h) w[h] = w[h + 1];
+        }
+#pragma unroll
+        for (int h = 0; h < Raw<T>::kWords; ++h) r.w[h] = __funnelshift_r(w[h], w[h + 1], bits);
     }
     return r;
 }
@@ -187,17 +205,22 @@ __device__ __forceinline__ void glu8(int kind, float (&v)[kVec], const float (&u
     }
 }
 
-// Block-wide maximum (of bits) and sum; `part` holds one word per warp.
-__device__ __forceinline__ uint32_t block_max(uint32_t v, uint32_t* part) {
+// Maximum (of bits) and sum over a row's threads: a warp (WARP) or the block;
+// `part` holds one word per warp.
+template <bool WARP>
+__device__ __forceinline__ uint32_t row_max(uint32_t v, uint32_t* part) {
     v = __reduce_max_sync(0xffffffffu, v);
+    if constexpr (WARP) return v;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = blockDim.x >> 5;
     if (lane == 0) part[warp] = v;
     __syncthreads();
     return __reduce_max_sync(0xffffffffu, lane < warps ? part[lane] : 0u);
 }
-__device__ __forceinline__ float block_sum(float v, float* part) {
+template <bool WARP>
+__device__ __forceinline__ float row_sum(float v, float* part) {
 #pragma unroll
     for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    if constexpr (WARP) return v;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = blockDim.x >> 5;
     if (lane == 0) part[warp] = v;
     __syncthreads();
@@ -256,18 +279,20 @@ __device__ __forceinline__ uint2 quantize8(const float (&v)[kVec], const Scale& 
 // VEC: rows of x and up start on 16-byte boundaries, rows of q on 8-byte ones.
 // At 64 registers and some 114 KB of a full SM's loads in flight, the loads of
 // other rows run while one is rounded.
-template <typename T, bool VEC, int PRO>
-__global__ void __launch_bounds__(kMaxThreads, 2) quantize_i8_kernel(const QuantizeI8 P) {
+template <typename T, bool VEC, int PRO, bool WARP>
+__global__ void __launch_bounds__(WARP ? kWarpRows * 32 : kMaxThreads, WARP ? 4 : 2) quantize_i8_kernel(const QuantizeI8 P) {
     constexpr int kKeep = keep_vecs(sizeof(T), PRO);
     __shared__ uint32_t part_max[kMaxThreads / 32];
     __shared__ float part_sum[kMaxThreads / 32];
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    const int64_t r = blockIdx.x;
+    const int64_t r = WARP ? static_cast<int64_t>(blockIdx.x) * kWarpRows + (threadIdx.x >> 5) : blockIdx.x;
+    if (WARP && r >= P.N) return;
     const T* x = static_cast<const T*>(P.x) + r * P.x_stride;
     const T* up = PRO == kProSwiglu ? static_cast<const T*>(P.up) + r * P.up_stride : nullptr;
     int8_t* q = P.q + r * P.q_stride;
-    const int K = P.K, vecs = K / kVec, step = blockDim.x;  // whole vectors; up to 7 values behind them
+    const int tid = WARP ? threadIdx.x & 31 : threadIdx.x;
+    const int K = P.K, vecs = K / kVec, step = WARP ? 32 : blockDim.x;  // whole vectors; up to 7 values behind them
     float rms = 1.f;
 
     // the prologue on a vector's or a single value
@@ -305,9 +330,10 @@ __global__ void __launch_bounds__(kMaxThreads, 2) quantize_i8_kernel(const Quant
         for (int j = 0; j < kVec; ++j) asm("max.NaN.f32 %0, %0, %1;" : "+f"(most) : "f"(fabsf(v[j])));
         return most;
     };
+    const bool wide = VEC || ((reinterpret_cast<uintptr_t>(P.q) | static_cast<uintptr_t>(P.q_stride)) & 7) == 0;
     auto store = [&](int i, const float (&v)[kVec], const Scale& c) {
         const uint2 w = quantize8(v, c);
-        if constexpr (VEC) {
+        if (wide) {
             *reinterpret_cast<uint2*>(q + static_cast<int64_t>(i) * kVec) = w;
         } else {
 #pragma unroll
@@ -323,7 +349,7 @@ __global__ void __launch_bounds__(kMaxThreads, 2) quantize_i8_kernel(const Quant
     if constexpr (PRO == kProNone) {
 #pragma unroll
         for (int c = 0; c < kKeep; ++c) {
-            const int i = threadIdx.x + c * step;
+            const int i = tid + c * step;
             if (i < vecs) raw[c] = load_vec<T, VEC>(x, i);
             else
 #pragma unroll
@@ -331,12 +357,12 @@ __global__ void __launch_bounds__(kMaxThreads, 2) quantize_i8_kernel(const Quant
         }
 #pragma unroll
         for (int c = 0; c < kKeep; ++c) top = max_raw<T>(top, raw[c]);
-        for (int i = threadIdx.x + kKeep * step; i < vecs; i += step) top = max_raw<T>(top, load_vec<T, VEC>(x, i));
+        for (int i = tid + kKeep * step; i < vecs; i += step) top = max_raw<T>(top, load_vec<T, VEC>(x, i));
         top = top_bits<T>(top);
     } else {
 #pragma unroll
         for (int c = 0; c < kKeep; ++c) {
-            const int i = threadIdx.x + c * step;
+            const int i = tid + c * step;
             if (i < vecs) value_at(i, keep[c]);
             else
 #pragma unroll
@@ -350,21 +376,21 @@ __global__ void __launch_bounds__(kMaxThreads, 2) quantize_i8_kernel(const Quant
             };
 #pragma unroll
             for (int c = 0; c < kKeep; ++c) add_vec(keep[c]);
-            for (int i = threadIdx.x + kKeep * step; i < vecs; i += step) {
+            for (int i = tid + kKeep * step; i < vecs; i += step) {
                 float v[kVec];
                 value_at(i, v);
                 add_vec(v);
             }
-            for (int k = vecs * kVec + threadIdx.x; k < K; k += step) sum = fmaf(single(k), single(k), sum);
-            rms = __fdiv_rn(1.f, __fsqrt_rn(__fadd_rn(__fdiv_rn(block_sum(sum, part_sum), static_cast<float>(K)), P.eps)));
+            for (int k = vecs * kVec + tid; k < K; k += step) sum = fmaf(single(k), single(k), sum);
+            rms = __fdiv_rn(1.f, __fsqrt_rn(__fadd_rn(__fdiv_rn(row_sum<WARP>(sum, part_sum), static_cast<float>(K)), P.eps)));
 #pragma unroll
             for (int c = 0; c < kKeep; ++c)
-                if (threadIdx.x + c * step < vecs) scaled_vec(threadIdx.x + c * step, keep[c]);
+                if (tid + c * step < vecs) scaled_vec(tid + c * step, keep[c]);
         }
         float most = 0.f;
 #pragma unroll
         for (int c = 0; c < kKeep; ++c) most = max_vec(most, keep[c]);
-        for (int i = threadIdx.x + kKeep * step; i < vecs; i += step) {
+        for (int i = tid + kKeep * step; i < vecs; i += step) {
             float v[kVec];
             value_at(i, v);
             scaled_vec(i, v);
@@ -372,17 +398,17 @@ __global__ void __launch_bounds__(kMaxThreads, 2) quantize_i8_kernel(const Quant
         }
         top = bits(most);
     }
-    for (int k = vecs * kVec + threadIdx.x; k < K; k += step) top = max(top, bits(scaled(k, single(k))));
-    top = block_max(top, part_max);
+    for (int k = vecs * kVec + tid; k < K; k += step) top = max(top, bits(scaled(k, single(k))));
+    top = row_max<WARP>(top, part_max);
 
     // ---- the scale
     const float a = __uint_as_float(top);
     const bool bad = top >= 0x7f800000u;  // NaN or infinity
     Scale c;
     c.s = bad ? __uint_as_float(0x7fc00000u) : __fdiv_rn(a, 127.f);
-    if (threadIdx.x == 0) P.scale[r] = c.s;
+    if (tid == 0) P.scale[r] = c.s;
     if (bad || a < 0x1p-100f) {
-        for (int k = threadIdx.x; k < K; k += step) q[k] = bad ? 0 : quantize_tiny(scaled(k, single(k)), c.s);
+        for (int k = tid; k < K; k += step) q[k] = bad ? 0 : quantize_tiny(scaled(k, single(k)), c.s);
         return;
     }
     const float inv = __fdiv_rn(1.f, c.s);
@@ -391,7 +417,7 @@ __global__ void __launch_bounds__(kMaxThreads, 2) quantize_i8_kernel(const Quant
     // ---- rounding
 #pragma unroll
     for (int n = 0; n < kKeep; ++n) {
-        const int i = threadIdx.x + n * step;
+        const int i = tid + n * step;
         if (i < vecs) {
             if constexpr (PRO == kProNone) {
                 float v[kVec];
@@ -402,19 +428,24 @@ __global__ void __launch_bounds__(kMaxThreads, 2) quantize_i8_kernel(const Quant
             }
         }
     }
-    for (int i = threadIdx.x + kKeep * step; i < vecs; i += step) {
+    for (int i = tid + kKeep * step; i < vecs; i += step) {
         float v[kVec];
         value_at(i, v);
         scaled_vec(i, v);
         store(i, v, c);
     }
-    for (int k = vecs * kVec + threadIdx.x; k < K; k += step) q[k] = quantize1(scaled(k, single(k)), c);
+    for (int k = vecs * kVec + tid; k < K; k += step) q[k] = quantize1(scaled(k, single(k)), c);
 }
 
-template <typename T, bool VEC>
+template <typename T, bool VEC, bool WARP>
 void (*pick(int kind))(QuantizeI8) {
-    return kind == kProNone ? quantize_i8_kernel<T, VEC, kProNone>
-                            : (kind == kProNorm ? quantize_i8_kernel<T, VEC, kProNorm> : quantize_i8_kernel<T, VEC, kProSwiglu>);
+    return kind == kProNone ? quantize_i8_kernel<T, VEC, kProNone, WARP>
+                            : (kind == kProNorm ? quantize_i8_kernel<T, VEC, kProNorm, WARP> : quantize_i8_kernel<T, VEC, kProSwiglu, WARP>);
+}
+template <typename T>
+void (*pick(bool vec, bool warp, int kind))(QuantizeI8) {
+    if (warp) return vec ? pick<T, true, true>(kind) : pick<T, false, true>(kind);
+    return vec ? pick<T, true, false>(kind) : pick<T, false, false>(kind);
 }
 
 }  // namespace
@@ -424,16 +455,16 @@ int launch_quantize_i8(const QuantizeI8& o, cudaStream_t stream) {
     uintptr_t bits = reinterpret_cast<uintptr_t>(o.x) | static_cast<uintptr_t>(o.x_stride * size);
     if (o.up) bits |= reinterpret_cast<uintptr_t>(o.up) | static_cast<uintptr_t>(o.up_stride * size);
     const bool vec = (bits & 15) == 0 && ((reinterpret_cast<uintptr_t>(o.q) | static_cast<uintptr_t>(o.q_stride)) & 7) == 0;
-    void (*kernel)(QuantizeI8) = nullptr;
-    if (o.x_type == kTypeF32) kernel = vec ? pick<float, true>(o.kind) : pick<float, false>(o.kind);
-    else if (o.x_type == kTypeF16) kernel = vec ? pick<__half, true>(o.kind) : pick<__half, false>(o.kind);
-    else kernel = vec ? pick<__nv_bfloat16, true>(o.kind) : pick<__nv_bfloat16, false>(o.kind);
-    const int parts = std::max(1, o.K / kVec);
-    const int keep = keep_vecs(size, o.kind);
-    const int want = o.N <= kFewRows ? parts : (parts + keep - 1) / keep;
-    const int threads = std::min(kMaxThreads, (want + 31) / 32 * 32);
+    // many rows that a warp's registers hold: a warp each
+    const int vecs = std::max(1, o.K / kVec), keep = keep_vecs(size, o.kind);
+    const bool warp = o.N > kFewRows && vecs <= 32 * keep;
+    void (*const kernel)(QuantizeI8) = o.x_type == kTypeF32   ? pick<float>(vec, warp, o.kind)
+                                       : o.x_type == kTypeF16 ? pick<__half>(vec, warp, o.kind)
+                                                              : pick<__nv_bfloat16>(vec, warp, o.kind);
+    const int want = o.N <= kFewRows ? vecs : (vecs + keep - 1) / keep;
+    const int threads = warp ? 32 * kWarpRows : std::min(kMaxThreads, (want + 31) / 32 * 32);
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(o.N);
+    cfg.gridDim = dim3(warp ? (o.N + kWarpRows - 1) / kWarpRows : o.N);
     cfg.blockDim = dim3(threads);
     cfg.stream = stream;
     cudaLaunchAttribute attr[1];

@@ -364,7 +364,7 @@ int combine(const MoeCombine& o, cudaStream_t stream) {
     const uintptr_t yb = reinterpret_cast<uintptr_t>(o.y) | static_cast<uintptr_t>(o.y_stride * ysize);
     const bool vec = o.M % N == 0 && ((zb | yb) & 15) == 0;
     const int64_t lanes = vec ? o.M / N : o.M;
-    const int threads = static_cast<int>(std::min<int64_t>(256, (lanes + 31) / 32 * 32));
+    const int threads = static_cast<int>(std::min<int64_t>(vec ? 256 : 128, (lanes + 31) / 32 * 32));
     const dim3 grid(static_cast<unsigned>((lanes + threads - 1) / threads), std::min(o.T, 65535));
     return vec ? launch(combine_kernel<T, N>, grid, threads, stream, o) : launch(combine_kernel<T, 1>, grid, threads, stream, o);
 }

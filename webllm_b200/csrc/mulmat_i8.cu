@@ -80,7 +80,7 @@ struct I8Args {
     CUtensorMap xmap;  // dense tokens: [rows][K] bytes, box 128 x the tile's rows of one CTA
     MulMatI8 o;
     int32_t tile_n;    // tokens of a full tile, a multiple of 16 (pair: of 32)
-    int32_t tiles_m, chunks, stages, splits;  // chunks: of a stage's bytes of K
+    int32_t tiles_m, tiles_n, chunks, stages, splits;  // tiles_n: dense; chunks: of a stage's bytes of K
     int32_t tmem_cols;
 };
 
@@ -343,19 +343,26 @@ struct Walk {
         constexpr int kStep = is_pair(MODE) ? 32 : 16;
         Item it;
         if constexpr (!GROUPED) {
-            const int tiles = (P.o.N + P.tile_n - 1) / P.tile_n;
+            const int c = P.tiles_n == 1 ? i : i / P.tiles_n;  // (no division for few tokens: an item may be 1000 clocks)
             it.e = 0;
-            it.m0 = i / tiles * kM;
-            it.first = i % tiles * P.tile_n;
+            it.m0 = c * kM;
+            it.first = (i - c * P.tiles_n) * P.tile_n;
             it.rows = min(P.tile_n, P.o.N - it.first);
         } else {
             while (cum[e + 1] * P.tiles_m <= i) ++e;
             const int tiles = cum[e + 1] - cum[e], j = i - cum[e] * P.tiles_m;
-            const int n = begin[e + 1] - begin[e], size = ((n + tiles - 1) / tiles + kStep - 1) / kStep * kStep;
+            const int n = begin[e + 1] - begin[e];
             it.e = e;
-            it.m0 = j / tiles * kM;
-            it.first = begin[e] + j % tiles * size;
-            it.rows = min(size, begin[e + 1] - it.first);
+            if (tiles == 1) {
+                it.m0 = j * kM;
+                it.first = begin[e];
+                it.rows = n;
+            } else {
+                const int c = j / tiles, size = ((n + tiles - 1) / tiles + kStep - 1) / kStep * kStep;
+                it.m0 = c * kM;
+                it.first = begin[e] + (j - c * tiles) * size;
+                it.rows = min(size, begin[e + 1] - it.first);
+            }
         }
         return it;
     }
@@ -387,14 +394,17 @@ __device__ __forceinline__ void store_tile(const MulMatI8& o, uint32_t taddr, in
                 } else {
                     const uint32_t own = half_pair(y, v), other = __shfl_xor_sync(0xffffffffu, own, 1);
                     // even lanes: column j of channels m, m + 1; odd: column j + 1 of m - 1, m
-                    const uint32_t w = lane & 1 ? __byte_perm(other, own, 0x7632) : __byte_perm(own, other, 0x5410);
+                    const uint32_t w = __byte_perm(own, other, lane & 1 ? 0x3276 : 0x5410);
                     *reinterpret_cast<uint32_t*>(y - (lane & 1) + at[n + j + (lane & 1)]) = w;
                 }
             }
         } else {
 #pragma unroll
-            for (int j = 0; j < 16; ++j)
-                if (n + j < rows && live) put(y + at[n + j], scaled(acc[j], s[n + j], tm));
+            for (int j = 0; j < 16; j += 2) {
+                const uint64_t v = scaled2(acc[j], acc[j + 1], *reinterpret_cast<const uint64_t*>(s + n + j), t2);
+                if (n + j < rows && live) put(y + at[n + j], low(v));
+                if (n + j + 1 < rows && live) put(y + at[n + j + 1], high(v));
+            }
         }
     }
 }
@@ -411,6 +421,7 @@ __global__ void __launch_bounds__(GROUPED ? kThreads + 2 * kLoaders : kThreads, 
     __shared__ int32_t warp_sum[(kThreads + 2 * kLoaders) / 32];
     __shared__ int64_t out_at[2][kTokens];  // where a tile's rows begin in y
     __shared__ __align__(8) float out_scale[2][kTokens];
+    static_assert(kTokens <= 32 * kEpiWarps, "a thread of the epilogue for each row of a tile");
     // 1024-byte alignment for the swizzled tiles
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     volatile int* poisoned = &poison;
@@ -497,7 +508,7 @@ __global__ void __launch_bounds__(GROUPED ? kThreads + 2 * kLoaders : kThreads, 
         __syncthreads();
         items = carry * P.tiles_m;
     } else {
-        items = (P.o.N + P.tile_n - 1) / P.tile_n * P.tiles_m;
+        items = P.tiles_n * P.tiles_m;
     }
     Walk<GROUPED, MODE> walk{P, cum, begin};
 
@@ -591,23 +602,50 @@ __global__ void __launch_bounds__(GROUPED ? kThreads + 2 * kLoaders : kThreads, 
         // ---------------- epilogue ----------------
         const int quad = warp & 3;                // the TMEM lanes this warp may read
         const int n0 = (warp - 2) / 4 % 2 * 16;   // it takes every other 16 columns, from here on
+        // An item's channel scale and, of the row that this thread looks after, the
+        // place in y and the scale are fetched while the item before it is stored.
+        const int mine = threadIdx.x - 64;
+        auto channel = [&](const Item& it) { return it.m0 + (PAIR ? kTileM * rank : 0) + 32 * quad + lane; };
+        auto fetch_channel = [&](const Item& it) {
+            const int m = channel(it);
+            return m < P.o.M ? P.o.w_scale[static_cast<int64_t>(it.e) * P.o.M + m] : 0.f;
+        };
+        auto fetch_row = [&](const Item& it) {
+            if (mine >= it.rows) return -1;
+            return GROUPED ? P.o.order[it.first + mine] : it.first + mine;
+        };
+        auto fetch_scale = [&](int row) { return row < 0 ? 0.f : P.o.q_scale[!GROUPED || P.o.per_slot ? row : row / P.o.k]; };
+        Item next{};
+        float next_tm = 0.f, next_scale = 0.f;
+        int next_row = -1;
+        if (item0 < items) {
+            next = walk.at(item0);
+            next_tm = fetch_channel(next);
+            next_row = fetch_row(next);
+            next_scale = fetch_scale(next_row);
+        }
         uint32_t t = 0;
         for (int i = item0; i < items; i += item_step, ++t) {
-            const Item it = walk.at(i);
+            const Item it = next;
             const uint32_t buf = t & 1;
-            const int m = it.m0 + (PAIR ? kTileM * rank : 0) + 32 * quad + lane;
-            const float tm = m < P.o.M ? P.o.w_scale[static_cast<int64_t>(it.e) * P.o.M + m] : 0.f;
-            for (int n = threadIdx.x - 64; n < it.rows; n += 32 * kEpiWarps) {
-                int row = it.first + n;
-                if constexpr (GROUPED) row = P.o.order[row];
-                out_at[buf][n] = row * P.o.y_stride;
-                out_scale[buf][n] = P.o.q_scale[!GROUPED || P.o.per_slot ? row : row / P.o.k];
+            const int m = channel(it);
+            const float tm = next_tm;
+            if (mine < it.rows) {
+                out_at[buf][mine] = next_row * P.o.y_stride;
+                out_scale[buf][mine] = next_scale;
+            }
+            const bool more = i + item_step < items;
+            if (more) {
+                next = walk.at(i + item_step);
+                next_tm = fetch_channel(next);
+                next_row = fetch_row(next);
             }
             asm volatile("bar.sync 1, %0;" ::"n"(32 * kEpiWarps) : "memory");  // the epilogue warps
             // after a time-out the items are still walked (the epilogue's warps meet at
             // the barrier above), without their stores
             const bool ok = mbar_wait(&acc_full[buf], (t >> 1) & 1, 2u, poisoned);
             tc_fence_after();
+            if (more) next_scale = fetch_scale(next_row);
             const uint32_t d = tmem + buf * P.tile_n + (static_cast<uint32_t>(32 * quad) << 16);
             if (!ok) {
             } else if constexpr (SPLIT) {
@@ -919,6 +957,7 @@ int launch(const MulMatI8& o, cudaStream_t stream, int num_sms) {
     const bool pair = is_pair(plan.mode);
     const int tile_m = pair ? 2 * kTileM : kTileM, sub = chunks_of_stage(plan.mode);
     P.tiles_m = (o.M + tile_m - 1) / tile_m;
+    P.tiles_n = GROUPED ? 0 : (o.N + P.tile_n - 1) / P.tile_n;
     P.chunks = (o.K + sub * kChunk - 1) / (sub * kChunk);
     const int tokens = pair ? P.tile_n / 2 : P.tile_n;  // of a CTA's stage
     const int stage_bytes = sub * (kABytes + tokens * kChunk);
