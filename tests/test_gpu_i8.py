@@ -106,7 +106,7 @@ def close(torch, y, ref, extra=0.0):
 
 @pytest.mark.parametrize("t", ["f32", "f16", "bf16"])
 @pytest.mark.parametrize("N,K", [(1, 1), (1, 7), (3, 64), (2, 255), (5, 1000), (1, 4096), (700, 333), (600, 4096), (2, 16384),
-                                 (1, 16385), (3, 40001), (530, 20000)])
+                                 (1, 16385), (3, 40001), (530, 20000), (700, 5), (1501, 1024), (3000, 2047), (513, 2064)])
 def test_quantize(rt, torch, t, N, K):
     g = gen_of(torch, "quantize", t, N, K)
     x = (torch.randn(N, K, device="cuda", generator=g) * torch.rand(N, 1, device="cuda", generator=g) * 5).to(types(torch)[t][0])
@@ -150,9 +150,13 @@ def test_quantize_extremes(rt, torch):
 @pytest.mark.parametrize("t", ["f32", "bf16"])
 @pytest.mark.parametrize("off,extra", [(0, 0), (1, 0), (0, 3), (8, 8)])
 def test_quantize_strides_and_alignment(rt, torch, t, off, extra):
-    """Rows at odd offsets and strides, a zero stride (one row for all), q rows back to back."""
-    N, K = 9, 203
-    g = gen_of(torch, "strides", t, off, extra)
+    """Rows at odd offsets and strides, a zero stride (one row for all), q rows back to back; a CTA a row and a warp a row."""
+    for N, K in ((9, 203), (601, 203)):
+        quantize_strided(torch, t, off, extra, N, K)
+
+
+def quantize_strided(torch, t, off, extra, N, K):
+    g = gen_of(torch, "strides", t, off, extra, N)
     dt, tt = types(torch)[t]
     flat = torch.randn(off + N * (K + extra), device="cuda", generator=g).to(dt)
     x = flat[off:].view(N, K + extra)[:, :K]
@@ -167,7 +171,7 @@ def test_quantize_strides_and_alignment(rt, torch, t, off, extra):
 
 
 @pytest.mark.parametrize("t", ["f32", "f16", "bf16"])
-@pytest.mark.parametrize("N,K", [(1, 96), (3, 1000), (600, 2048), (2, 20000)])
+@pytest.mark.parametrize("N,K", [(1, 96), (3, 1000), (600, 333), (600, 2048), (2, 20000)])
 def test_quantize_rms_norm(rt, torch, t, N, K):
     """|q - v / s| <= 1/2 and s = max|v| / 127, v off by eps: the sum of squares (at most 40 terms a thread at these
     sizes, then a tree of 10), a mean, a root, a reciprocal and two products: 64 u(f32)."""
@@ -184,7 +188,7 @@ def test_quantize_rms_norm(rt, torch, t, N, K):
 
 @pytest.mark.parametrize("t", ["f32", "f16", "bf16"])
 @pytest.mark.parametrize("kind", [jsep.GLU_SWIGLU, jsep.GLU_GELU])
-@pytest.mark.parametrize("N,K", [(1, 72), (5, 1001), (600, 512)])
+@pytest.mark.parametrize("N,K", [(1, 72), (5, 1001), (600, 512), (600, 333), (520, 1500)])
 def test_quantize_glu(rt, torch, t, kind, N, K):
     """act(g) u within eps |v| + tiny: __expf is off by 2 + 1.16 |g| ulp, |g| <= 20, the division by 2 ulp and the rest
     by 2: 30 ulp = 60 u(f32). GELU is an f16 number: at most one step (2^-10, or 2^-24 below the normals) beside."""
