@@ -250,7 +250,9 @@ def _own(st):
         jsep.mul_mat_i8(w.data_ptr(), pitch, t.data_ptr(), q.data_ptr(), pitch, s.data_ptr(), types[st["y"]], y.data_ptr(), M, M, K, rows, stream=stream)
         return y
     T, k, up = st["T"], st["k"], st["part"] == "up"
-    tz = types[st["y"]] if up else jsep.GGML_TYPE_F16  # the slots' rows ahead of their sum: 11 bits where the sum keeps 8
+    tz = types[st["y"]]
+    if not up:  # the slots' rows stay in 32 bits ahead of their sum: in 16 they would be rounded twice, and f16 ends at 65504
+        y, tz = y.new_empty(y.shape, dtype=torch.float32), jsep.GGML_TYPE_F32
     jsep.mul_mat_id_i8(w.data_ptr(), pitch, M * pitch, t.data_ptr(), q.data_ptr(), pitch, s.data_ptr(), not up, st["offsets"].data_ptr(), st["order"].data_ptr(),
                        tz, y.data_ptr(), M, M, K, st["E"], T, k, stream=stream)
     if up:
