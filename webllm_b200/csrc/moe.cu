@@ -382,18 +382,19 @@ int launch_moe_plan(const int32_t* ids, int64_t slots, int E, int32_t* offsets, 
     const int warps = static_cast<int>(std::min<int64_t>(kPlanWarps, want));
     const int ctas = static_cast<int>(std::min<int64_t>(kPlanCtas, (want + kPlanWarps - 1) / kPlanWarps));
     const int smem = (warps + 2) * (E + 1) * 4;
-    if (smem > 48 * 1024 || ctas > 8) {
-        static bool configured[kMaxDevices] = {};  // the attribute is per device
-        int dev = 0;
-        if (const cudaError_t e = cudaGetDevice(&dev); e != cudaSuccess) return -static_cast<int>(e);
-        if (dev < 0 || dev >= kMaxDevices) return -static_cast<int>(cudaErrorInvalidDevice);
-        if (!configured[dev]) {
-            cudaError_t e = cudaFuncSetAttribute(plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                                 (kPlanWarps + 2) * (kMaxExperts + 1) * 4);
-            if (e == cudaSuccess) e = cudaFuncSetAttribute(plan_kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
-            if (e != cudaSuccess) return -static_cast<int>(e);
-            configured[dev] = true;
-        }
+    // The attributes are per device, and set ahead of its first launch whatever that
+    // one needs: static shared memory counts against the 48 KB that a launch has
+    // without them, so the dynamic size alone does not tell.
+    static bool configured[kMaxDevices] = {};
+    int dev = 0;
+    if (const cudaError_t e = cudaGetDevice(&dev); e != cudaSuccess) return -static_cast<int>(e);
+    if (dev < 0 || dev >= kMaxDevices) return -static_cast<int>(cudaErrorInvalidDevice);
+    if (!configured[dev]) {
+        cudaError_t e = cudaFuncSetAttribute(plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                             (kPlanWarps + 2) * (kMaxExperts + 1) * 4);
+        if (e == cudaSuccess) e = cudaFuncSetAttribute(plan_kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+        if (e != cudaSuccess) return -static_cast<int>(e);
+        configured[dev] = true;
     }
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(ctas);
