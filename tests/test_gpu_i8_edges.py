@@ -6,11 +6,54 @@ import os
 import subprocess
 import sys
 
+import zlib
+
 import pytest
+
+from webllm_b200 import jsep
 
 pytestmark = pytest.mark.gpu
 
+U32 = 2.0 ** -24  # half a step of an f32, relative
 REPO = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+
+
+@pytest.fixture(scope="module")
+def torch():
+    import torch
+
+    return torch
+
+
+@pytest.fixture(scope="module")
+def rt(runtime):
+    return runtime
+
+
+def here(torch):
+    return torch.cuda.current_stream().cuda_stream or jsep.STREAM_LEGACY
+
+
+def up16(n):
+    return (n + 15) // 16 * 16
+
+
+def gen_of(torch, *key):
+    g = torch.Generator(device="cuda")
+    g.manual_seed(zlib.crc32(repr(key).encode()))
+    return g
+
+
+def quantize(torch, x, **kw):
+    """q and scales of the rows of x through the library."""
+    N, K = x.shape
+    q = torch.full((N, up16(K)), 77, dtype=torch.int8, device="cuda")
+    s = torch.full((N,), -1.0, device="cuda")
+    t = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 30}[x.dtype]
+    jsep.quantize_i8(t, x.data_ptr(), x.stride(0), N, K, q.data_ptr(), q.stride(0), s.data_ptr(), stream=here(torch), **kw)
+    torch.cuda.synchronize()
+    assert (q[:, K:] == 77).all(), "bytes behind a row were written"
+    return q[:, :K], s
 
 
 def run_fresh(code, *args):
@@ -43,3 +86,40 @@ def test_first_plan_of_a_process(slots, E):
     """Sizes whose shared memory is within 48 KB only without what the kernel holds statically: as the first plan of a
     process (a larger one before it raises the kernel's limit for the rest)."""
     run_fresh(FIRST_PLAN, slots, E)
+
+
+# ---------------------------------------------------------------- quantiser
+
+
+@pytest.mark.parametrize("t", ["float32", "bfloat16"])
+@pytest.mark.parametrize("N,K", [(1, 5), (3, 1001), (2, 20000), (600, 333), (700, 64)])
+def test_rms_norm_of_any_finite_row(rt, torch, t, N, K):
+    """Rows whose squares overflow an f32 or fall below its normals, among ordinary ones: x / sqrt(mean(x^2) + eps) is of
+    order 1 for all of them. |q - v / s| <= 1/2 and s = max|v| / 127 with v off by eps: what test_quantize_rms_norm allows
+    for f32 sums (64 u); the sums of these rows are doubles."""
+    g = gen_of(torch, "far", t, N, K)
+    eps = 64 * U32
+    for e in (1e-5, 0.0):
+        # by rows: ordinary, squares past the largest f32, and near the largest value; with eps = 0 tiny ones too
+        sizes = [1.0, 1e20, 3e37, 1e30] + ([1e-21, 1e-25, 1e-37] if e == 0 else [])
+        size = torch.tensor(sizes, device="cuda", dtype=torch.float64)[torch.arange(N, device="cuda") % len(sizes)]
+        x = (torch.randn(N, K, device="cuda", generator=g).clamp(-4, 4).double() * size[:, None]).to(getattr(torch, t))
+        for gain in (None, torch.rand(K, device="cuda", generator=g) + 0.5):
+            q, s = quantize(torch, x, rms_norm=True, gain_ptr=0 if gain is None else gain.data_ptr(), eps=e)
+            xd = x.double()
+            v = xd / (xd.square().mean(1, keepdim=True) + e).sqrt() * (1.0 if gain is None else gain.double())
+            assert ((s.double() * 127 / v.abs().amax(1) - 1).abs() <= eps + 2 * U32).all()
+            assert ((q.double() - v / s.double()[:, None]).abs() <= 0.5 + 127 * (eps + 2 * U32)).all()
+
+
+@pytest.mark.parametrize("size", [1.0, 1e25])
+@pytest.mark.parametrize("N", [4, 604])
+def test_rms_norm_of_rows_with_nan_or_infinity(rt, torch, N, size):
+    """Such a row has scale NaN and q = 0; the rows beside it have theirs."""
+    x = torch.randn(N, 300, device="cuda", generator=gen_of(torch, "bad", N)) * size
+    alone = quantize(torch, x, rms_norm=True, eps=1e-6)
+    x[1, 7], x[2, 299] = float("nan"), -float("inf")
+    q, s = quantize(torch, x, rms_norm=True, eps=1e-6)
+    assert torch.isnan(s[1:3]).all() and (q[1:3] == 0).all()
+    keep = [n for n in range(N) if n not in (1, 2)]
+    assert torch.equal(q[keep], alone[0][keep]) and torch.equal(s[keep], alone[1][keep]) and torch.isfinite(s[keep]).all()

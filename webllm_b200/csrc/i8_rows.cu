@@ -293,7 +293,7 @@ __global__ void __launch_bounds__(WARP ? kWarpRows * 32 : kMaxThreads, WARP ? 4 
     int8_t* q = P.q + r * P.q_stride;
     const int tid = WARP ? threadIdx.x & 31 : threadIdx.x;
     const int K = P.K, vecs = K / kVec, step = WARP ? 32 : blockDim.x;  // whole vectors; up to 7 values behind them
-    float rms = 1.f;
+    float rms = 1.f, pre = 1.f;  // behind RMS_NORM: 1 / rms, and what x is multiplied by ahead of it
 
     // the prologue on a vector's or a single value
     auto value = [&](const Raw<T>& a, const Raw<T>& b, float (&v)[kVec]) {
@@ -302,6 +302,10 @@ __global__ void __launch_bounds__(WARP ? kWarpRows * 32 : kMaxThreads, WARP ? 4 
             float u[kVec];
             unpack<T>(b, u);
             glu8(P.kind, v, u);
+        }
+        if constexpr (PRO == kProNorm) {
+#pragma unroll
+            for (int j = 0; j < kVec; ++j) v[j] *= pre;
         }
     };
     auto value_at = [&](int i, float (&v)[kVec]) {
@@ -321,6 +325,7 @@ __global__ void __launch_bounds__(WARP ? kWarpRows * 32 : kMaxThreads, WARP ? 4 
     };
     auto single = [&](int k) {
         const float v = to_f32(x[k]);
+        if constexpr (PRO == kProNorm) return v * pre;
         return PRO == kProSwiglu ? glu(P.kind, v, to_f32(up[k])) : v;
     };
     auto bits = [](float v) { return __float_as_uint(v) & 0x7fffffffu; };
@@ -369,20 +374,37 @@ __global__ void __launch_bounds__(WARP ? kWarpRows * 32 : kMaxThreads, WARP ? 4 
                 for (int j = 0; j < kVec; ++j) keep[c][j] = 0.f;
         }
         if constexpr (PRO == kProNorm) {
-            float sum = 0.f;
-            auto add_vec = [&](const float (&v)[kVec]) {
+            auto square_sum = [&] {
+                float sum = 0.f;
+                auto add_vec = [&](const float (&v)[kVec]) {
 #pragma unroll
-                for (int j = 0; j < kVec; ++j) sum = fmaf(v[j], v[j], sum);
+                    for (int j = 0; j < kVec; ++j) sum = fmaf(v[j], v[j], sum);
+                };
+#pragma unroll
+                for (int c = 0; c < kKeep; ++c) add_vec(keep[c]);
+                for (int i = tid + kKeep * step; i < vecs; i += step) {
+                    float v[kVec];
+                    value_at(i, v);
+                    add_vec(v);
+                }
+                for (int k = vecs * kVec + tid; k < K; k += step) sum = fmaf(single(k), single(k), sum);
+                return row_sum<WARP>(sum, part_sum);
             };
+            const float mean = __fadd_rn(__fdiv_rn(square_sum(), static_cast<float>(K)), P.eps);
+            if (mean >= 0x1p-100f && mean <= 3.402823466e38f) {
+                rms = __fdiv_rn(1.f, __fsqrt_rn(mean));
+            } else {
+                // Squares past the largest f32, or (with an eps of next to nothing) so small
+                // that what was lost below the normals counts: x * 2^-96 or x * 2^96
+                // instead, exact but for values that are nothing beside the row's others.
+                pre = mean < 1.f ? 0x1p96f : 0x1p-96f;
 #pragma unroll
-            for (int c = 0; c < kKeep; ++c) add_vec(keep[c]);
-            for (int i = tid + kKeep * step; i < vecs; i += step) {
-                float v[kVec];
-                value_at(i, v);
-                add_vec(v);
+                for (int c = 0; c < kKeep; ++c)
+#pragma unroll
+                    for (int j = 0; j < kVec; ++j) keep[c][j] *= pre;
+                if constexpr (!WARP) __syncthreads();  // the first sum's parts have been read
+                rms = static_cast<float>(1.0 / sqrt(static_cast<double>(square_sum()) / K + static_cast<double>(P.eps) * pre * pre));
             }
-            for (int k = vecs * kVec + tid; k < K; k += step) sum = fmaf(single(k), single(k), sum);
-            rms = __fdiv_rn(1.f, __fsqrt_rn(__fadd_rn(__fdiv_rn(row_sum<WARP>(sum, part_sum), static_cast<float>(K)), P.eps)));
 #pragma unroll
             for (int c = 0; c < kKeep; ++c)
                 if (tid + c * step < vecs) scaled_vec(tid + c * step, keep[c]);
