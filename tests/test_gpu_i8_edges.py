@@ -123,3 +123,33 @@ def test_rms_norm_of_rows_with_nan_or_infinity(rt, torch, N, size):
     assert torch.isnan(s[1:3]).all() and (q[1:3] == 0).all()
     keep = [n for n in range(N) if n not in (1, 2)]
     assert torch.equal(q[keep], alone[0][keep]) and torch.equal(s[keep], alone[1][keep]) and torch.isfinite(s[keep]).all()
+
+
+@pytest.mark.parametrize("t", ["float32", "float16", "bfloat16"])
+@pytest.mark.parametrize("off", [0, 1])
+@pytest.mark.parametrize("N,K", [(1, 8), (3, 1001), (2, 20000), (600, 333), (700, 64)])
+def test_swiglu_of_gates_far_below_zero(rt, torch, t, off, N, K):
+    """silu(g) u of rows whose gates all lie between -70 and -130: s = max|v| / 127 and |q - v / s| <= 1/2 with v off by eps.
+    e^g by the SFU: its argument g log2(e) is off by u |g| log2(e), which is u |g| of the result, and each of at most four
+    factors by 2 ulp = 4 u; five products and 1 + e^-g by u each: u (130 + 16 + 6), and what is below f32's normals by
+    half a step of theirs (2^-150). s too may be below them: then it is off from a / 127 by up to 2^-150, and the value at
+    q = 127, the largest, by 127 times that."""
+    g = gen_of(torch, "deep", t, off, N, K)
+    dt = getattr(torch, t)
+    low = 60.0 * torch.rand(N, 1, device="cuda", generator=g)  # a row's gates within 8 of each other
+    gate = (-70 - low - 8 * torch.rand(N, K + off, device="cuda", generator=g)).clamp(min=-130).to(dt)[:, off:]
+    up = (torch.randn(N, K, device="cuda", generator=g) * (1e4 if t == "float16" else 1e30)).clamp(-6e4 if t == "float16" else -3e38, 6e4 if t == "float16" else 3e38).to(dt)
+    x = gate.contiguous() if off == 0 else gate
+    tt = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 30}[dt]
+    q, s = torch.zeros(N, K, dtype=torch.int8, device="cuda"), torch.zeros(N, device="cuda")
+    jsep.quantize_i8(tt, x.data_ptr(), x.stride(0), N, K, q.data_ptr(), K, s.data_ptr(), glu=jsep.GLU_SWIGLU, up_ptr=up.data_ptr(), up_stride=K,
+                     stream=here(torch))
+    torch.cuda.synchronize()
+    gd = gate.double()
+    v = gd / (1 + (-gd).exp()) * up.double()
+    eps, sub = (130 + 16 + 6) * U32, 2.0 ** -150
+    top, sd = v.abs().amax(1), s.double()
+    assert ((sd * 127 - top).abs() <= (eps + 2 * U32) * top + 4 * sub + 127 * sub).all()
+    live = sd > 0
+    assert (q[~live] == 0).all() and (top[~live] <= 127 * sub * 2).all()
+    assert ((q.double() * sd[:, None] - v).abs() <= 0.5 * sd[:, None] + eps * v.abs() + 127 * sd[:, None] * 2 * U32 + (127 + 6) * sub).all()

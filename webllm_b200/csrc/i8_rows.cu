@@ -169,13 +169,38 @@ __device__ __forceinline__ float rcp(float x) {
 }
 
 // silu(g) * u and gelu(g) * u, as wllm_mul_mat_glu_batch computes them: x / (1 +
-// e^-z) with the SFU's exponential and reciprocal. What they flush to zero (an
-// e^-z below 2^-126, a reciprocal of more than 2^126) is lost in the sum or the
-// product anyway.
+// e^-z) with the SFU's exponential and reciprocal. Both flush results below the
+// normals to zero: an e^-z below 2^-126 is lost in the sum anyway, but a
+// reciprocal of more than 2^126 (a gate below some -87) is not, since u, or a row
+// whose gates are all so small, brings it back. A row with a gate below kDeep is
+// computed value by value, such gates' with silu_deep.
 constexpr float kLog2e = 1.4426950408889634f;
 __device__ __forceinline__ float x_sigmoid(float x, float z) { return x * rcp(1.f + ex2(z * -kLog2e)); }
+constexpr float kDeep = -87.f;
+// There 1 + e^-g is e^-g to the last bit: g e^g u, e^g in four factors that stay
+// normal wherever the product can.
+__device__ __forceinline__ float silu_deep(float g, float u) {
+    const float h = ex2(g * (0.25f * kLog2e));
+    return g * h * h * u * h * h;
+}
+// The bits of a vector's lowest gate, where it is negative (there the bits order by
+// size, above all positive ones), and whether they are below kDeep.
+template <typename T>
+__device__ __forceinline__ uint32_t lowest(uint32_t most, const Raw<T>& r) {
+#pragma unroll
+    for (int h = 0; h < Raw<T>::kWords; ++h) {
+        if constexpr (sizeof(T) == 4) most = max(most, r.w[h]);
+        else most = __vmaxu2(most, r.w[h]);
+    }
+    return most;
+}
+template <typename T>
+__device__ __forceinline__ bool is_deep(uint32_t most) {
+    if constexpr (sizeof(T) == 4) return most > 0xC2AE0000u;
+    return max(most & 0xffffu, most >> 16) > (std::is_same<T, __half>::value ? 0xD570u : 0xC2AEu);
+}
 __device__ __forceinline__ float glu(int kind, float g, float u) {
-    if (kind == kProSwiglu) return __fmul_rn(x_sigmoid(g, g), u);
+    if (kind == kProSwiglu) return g < kDeep ? silu_deep(g, u) : __fmul_rn(x_sigmoid(g, g), u);
     float y;
     if (g <= -10.f) {
         y = 0.f;
@@ -247,8 +272,9 @@ __device__ __forceinline__ uint32_t nearest(float v, float s, uint32_t lo, uint3
 __device__ __forceinline__ int8_t quantize1(float v, const Scale& c) {
     return static_cast<int8_t>(nearest(v, c.s, __float_as_uint(fmaf(v, c.lo, kMagic)), __float_as_uint(fmaf(v, c.hi, kMagic))));
 }
-// In a row of tiny values, where 1/s could overflow.
-__device__ __forceinline__ int8_t quantize_tiny(float v, float s) {
+// In a row of tiny values, where 1/s could overflow, or one that is computed value
+// by value.
+__device__ __forceinline__ int8_t quantize_exact(float v, float s) {
     return s > 0.f ? static_cast<int8_t>(fmin(fmax(rint(static_cast<double>(v) / s), -127.0), 127.0)) : 0;
 }
 
@@ -308,8 +334,10 @@ __global__ void __launch_bounds__(WARP ? kWarpRows * 32 : kMaxThreads, WARP ? 4 
             for (int j = 0; j < kVec; ++j) v[j] *= pre;
         }
     };
+    uint32_t low_gate = 0;  // lowest() of this thread's gates
     auto value_at = [&](int i, float (&v)[kVec]) {
         const Raw<T> a = load_vec<T, VEC>(x, i);
+        if constexpr (PRO == kProSwiglu) low_gate = lowest(low_gate, a);
         value(a, PRO == kProSwiglu ? load_vec<T, VEC>(up, i) : a, v);
     };
     auto scaled = [&](int k, float v) {
@@ -421,7 +449,16 @@ __global__ void __launch_bounds__(WARP ? kWarpRows * 32 : kMaxThreads, WARP ? 4 
         top = bits(most);
     }
     for (int k = vecs * kVec + tid; k < K; k += step) top = max(top, bits(scaled(k, single(k))));
+    // the sign bit, above all maxima: this row has a gate that glu8 does not hold for
+    if (PRO == kProSwiglu && P.kind == kProSwiglu && is_deep<T>(low_gate)) top |= 0x80000000u;
     top = row_max<WARP>(top, part_max);
+    const bool deep = PRO == kProSwiglu && (top >> 31);
+    if (deep) {
+        top = 0;
+        for (int k = tid; k < K; k += step) top = max(top, bits(single(k)));
+        if constexpr (!WARP) __syncthreads();  // part_max has been read
+        top = row_max<WARP>(top, part_max);
+    }
 
     // ---- the scale
     const float a = __uint_as_float(top);
@@ -429,8 +466,8 @@ __global__ void __launch_bounds__(WARP ? kWarpRows * 32 : kMaxThreads, WARP ? 4 
     Scale c;
     c.s = bad ? __uint_as_float(0x7fc00000u) : __fdiv_rn(a, 127.f);
     if (tid == 0) P.scale[r] = c.s;
-    if (bad || a < 0x1p-100f) {
-        for (int k = tid; k < K; k += step) q[k] = bad ? 0 : quantize_tiny(scaled(k, single(k)), c.s);
+    if (bad || a < 0x1p-100f || deep) {
+        for (int k = tid; k < K; k += step) q[k] = bad ? 0 : quantize_exact(scaled(k, single(k)), c.s);
         return;
     }
     const float inv = __fdiv_rn(1.f, c.s);
