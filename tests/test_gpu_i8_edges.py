@@ -153,3 +153,55 @@ def test_swiglu_of_gates_far_below_zero(rt, torch, t, off, N, K):
     live = sd > 0
     assert (q[~live] == 0).all() and (top[~live] <= 127 * sub * 2).all()
     assert ((q.double() * sd[:, None] - v).abs() <= 0.5 * sd[:, None] + eps * v.abs() + 127 * sd[:, None] * 2 * U32 + (127 + 6) * sub).all()
+
+
+# ---------------------------------------------------------------- grouped product
+
+
+def grouped(torch, w, ws, q, qs, per_slot, ids, M, K, t="float32"):
+    """The grouped product of ids [T][k] through the library's plan, and that plan."""
+    (T, k), E = ids.shape, ws.shape[0]
+    offsets, order = torch.empty(E + 1, dtype=torch.int32, device="cuda"), torch.empty(T * k, dtype=torch.int32, device="cuda")
+    y = torch.full((T * k, M), float("nan"), dtype=getattr(torch, t), device="cuda")
+    st = here(torch)
+    jsep.moe_plan(ids.data_ptr(), T, k, E, offsets.data_ptr(), order.data_ptr(), stream=st)
+    jsep.mul_mat_id_i8(w.data_ptr(), w.stride(1), w.stride(0), ws.data_ptr(), q.data_ptr(), q.stride(0), qs.data_ptr(), per_slot, offsets.data_ptr(),
+                       order.data_ptr(), {"float32": 0, "float16": 1, "bfloat16": 30}[t], y.data_ptr(), M, M, K, E, T, k, stream=st)
+    torch.cuda.synchronize()
+    return y
+
+
+def ref_grouped(torch, w, ws, q, qs, per_slot, ids, K):
+    (T, k), flat = ids.shape, ids.flatten()
+    y = torch.zeros(T * k, ws.shape[1], dtype=torch.float64, device="cuda")
+    for e in flat.unique().tolist():
+        if 0 <= e < ws.shape[0]:
+            at = (flat == e).nonzero().flatten()
+            row = at if per_slot else at // k
+            y[at] = (q[row, :K].double() @ w[e, :, :K].double().t()) * qs[row].double()[:, None] * ws[e].double()
+    return y
+
+
+def close(torch, y, ref):
+    """The sum is exact: acc -> f32, two f32 products and the rounding to y's type."""
+    u = {torch.float32: 0.0, torch.float16: 2.0 ** -11, torch.bfloat16: 2.0 ** -8}[y.dtype]
+    sub = 2.0 ** -25 if y.dtype == torch.float16 else 0.0
+    bad = ~((y.double() - ref).abs() <= (3.01 * U32 + 1.001 * u) * ref.abs() + sub)
+    assert not bad.any(), f"{int(bad.sum())} of {bad.numel()} off, first {bad.nonzero()[0].tolist()}"
+
+
+@pytest.mark.parametrize("per_slot", [False, True])
+@pytest.mark.parametrize("K", [1, 15, 17, 127, 129, 130, 255, 257, 1000, 1535])
+def test_grouped_rows_that_end_inside_a_piece(rt, torch, per_slot, K):
+    """Every row's last 16 bytes partly behind K, the last row at the end of its buffer, with marks behind each row."""
+    T, k, E, M = 61, 3, 7, 140
+    g = gen_of(torch, "pieces", K, per_slot)
+    pitch = up16(K)
+    rows = T * k if per_slot else T
+    w = torch.randint(-127, 128, (E, M, pitch), dtype=torch.int8, device="cuda", generator=g)
+    ws, qs = torch.rand(E, M, device="cuda", generator=g), torch.rand(rows, device="cuda", generator=g)
+    flat = torch.full(((rows - 1) * pitch + K,), 99, dtype=torch.int8, device="cuda")  # nothing behind the last row's K values
+    q = flat.as_strided((rows, K), (pitch, 1))
+    q.copy_(torch.randint(-127, 128, (rows, K), dtype=torch.int8, device="cuda", generator=g))
+    ids = torch.randint(-1, E, (T, k), dtype=torch.int32, device="cuda", generator=g)
+    close(torch, grouped(torch, w, ws, q, qs, per_slot, ids, M, K), ref_grouped(torch, w, ws, q, qs, per_slot, ids, K))

@@ -22,7 +22,7 @@ LIB_PATH = os.path.join(PKG_DIR, "libwllm_mulmat.so")
 
 SOURCES = ["runtime.cpp", "mulmat_gemv.cu", "mulmat_stream.cu", "mulmat_prefill.cu", "mulmat_batched.cu",
            "mulmat_batched_tc.cu", "i8_rows.cu", "mulmat_i8.cu", "moe.cu"]
-HEADERS = ["wllm_internal.h", "quant_blocks.cuh"]
+HEADERS = ["wllm_internal.h", "quant_blocks.cuh", "i8_plan.h"]
 ARCH_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a"]
 
 

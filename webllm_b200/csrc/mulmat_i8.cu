@@ -54,6 +54,7 @@
 #include <algorithm>
 #include <cmath>
 
+#include "i8_plan.h"
 #include "wllm_internal.h"
 
 namespace wllm {
@@ -167,7 +168,7 @@ __device__ __forceinline__ void tma_3d_pair(uint32_t dst, const CUtensorMap* tm,
         "l"(tm), "r"(x), "r"(y), "r"(z), "r"(smem_u32(bar) & 0xFEFFFFFFu), "l"(policy)
         : "memory");
 }
-// 16 bytes to shared memory, zeros where bytes is 0.
+// 16 bytes to shared memory: `bytes` of src, then zeros.
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, uint32_t bytes) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
 }
@@ -719,12 +720,12 @@ __global__ void __launch_bounds__(GROUPED ? kThreads + 2 * kLoaders : kThreads, 
                 ok = q < stages || mbar_wait(&empty[s], ring.parity ^ 1, 1u, poisoned);
                 ok = __all_sync(0xffffffffu, ok);
                 if (!ok) break;
-                // piece p of row r lies at r * 128 + (p ^ (r % 8)) * 16; bytes behind K, where
-                // the weights are zeros, may hold anything, but nothing is read behind the row
+                // piece p of row r lies at r * 128 + (p ^ (r % 8)) * 16; of the last piece only
+                // the row's own bytes are read, and zeros stand behind them
 #pragma unroll
                 for (int h = 0; h < kSub; ++h) {
                     const int k = (c * kSub + h) * kChunk + piece * 16;
-                    const uint32_t bytes = k < P.o.K ? 16 : 0;
+                    const uint32_t bytes = piece_bytes(P.o.K, k);
                     const int at = k < P.o.K ? k : 0;
                     const uint32_t dst = smem_u32(smem + s * stage_bytes) + kSub * kABytes + h * b_bytes + r0 * kChunk + ((piece ^ (r0 & 7)) << 4);
 #pragma unroll
