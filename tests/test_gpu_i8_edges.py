@@ -88,6 +88,17 @@ def test_first_plan_of_a_process(slots, E):
     run_fresh(FIRST_PLAN, slots, E)
 
 
+FIRST_PLAN_CAPTURED = FIRST_PLAN.replace("jsep.moe_plan(", """graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    jsep.moe_plan(""").replace("stream=jsep.STREAM_LEGACY)", "stream=torch.cuda.current_stream().cuda_stream)\ngraph.replay()")
+
+
+@pytest.mark.parametrize("slots,E", [(65536, 128), (40000, 1024)])
+def test_first_plan_of_a_process_is_captured(slots, E):
+    """A plan of many CTAs, whose cluster size is looked up in the same call, while a stream is being captured."""
+    run_fresh(FIRST_PLAN_CAPTURED, slots, E)
+
+
 # ---------------------------------------------------------------- quantiser
 
 

@@ -8,6 +8,7 @@
 #include <algorithm>
 #include <type_traits>
 
+#include "i8_plan.h"
 #include "wllm_internal.h"
 
 namespace wllm {
@@ -113,9 +114,6 @@ __global__ void __launch_bounds__(32 * kRouteWarps) route_kernel(const MoeRoute 
 // keys in their order (they find each other with a ballot for each bit). Bound:
 // latency (8 T k bytes are moved): 10 us for 65,536 slots and 128 experts, 4 for
 // 8 slots; a CTA per expert that read all ids took 26, 8 CTAs 17.
-constexpr int kPlanWarps = 32;
-constexpr int kPlanCtas = 16;  // at most
-
 constexpr int kPlanBatch = 8;   // ids a lane fetches at once
 
 __device__ __forceinline__ int plan_key(const int32_t* ids, int64_t i, int64_t end, int E) {
@@ -376,38 +374,44 @@ int launch_moe_route(const MoeRoute& o, cudaStream_t stream) {
 }
 
 int launch_moe_plan(const int32_t* ids, int64_t slots, int E, int32_t* offsets, int32_t* order, cudaStream_t stream) {
-    // 64 slots a warp before there is another warp (four at least, for the walks
-    // over the keys), all warps of a CTA before another CTA
-    const int64_t want = std::max<int64_t>(4, (slots + 63) / 64);
-    const int warps = static_cast<int>(std::min<int64_t>(kPlanWarps, want));
-    const int ctas = static_cast<int>(std::min<int64_t>(kPlanCtas, (want + kPlanWarps - 1) / kPlanWarps));
-    const int smem = (warps + 2) * (E + 1) * 4;
-    // The attributes are per device, and set ahead of its first launch whatever that
-    // one needs: static shared memory counts against the 48 KB that a launch has
-    // without them, so the dynamic size alone does not tell.
-    static bool configured[kMaxDevices] = {};
     int dev = 0;
     if (const cudaError_t e = cudaGetDevice(&dev); e != cudaSuccess) return -static_cast<int>(e);
     if (dev < 0 || dev >= kMaxDevices) return -static_cast<int>(cudaErrorInvalidDevice);
-    if (!configured[dev]) {
-        cudaError_t e = cudaFuncSetAttribute(plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                             (kPlanWarps + 2) * (kMaxExperts + 1) * 4);
-        if (e == cudaSuccess) e = cudaFuncSetAttribute(plan_kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
-        if (e != cudaSuccess) return -static_cast<int>(e);
-        configured[dev] = true;
-    }
+    // The kernel's attributes are per device, and set ahead of its first launch
+    // whatever that one needs: static shared memory counts against the 48 KB that a
+    // launch has without them, so the dynamic size alone does not tell.
+    static int most_ctas[kMaxDevices] = {};
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(ctas);
-    cfg.blockDim = dim3(32 * warps);
-    cfg.dynamicSmemBytes = smem;
     cfg.stream = stream;
     cudaLaunchAttribute attr[2];
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
-    attr[1].id = cudaLaunchAttributeClusterDimension;
-    attr[1].val.clusterDim.x = static_cast<unsigned>(ctas);
-    attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
+    if (most_ctas[dev] == 0) {
+        const int smem = plan_smem(kPlanWarps, kMaxExperts);
+        cudaError_t e = cudaFuncSetAttribute(plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+        if (e == cudaSuccess) e = cudaFuncSetAttribute(plan_kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+        if (e != cudaSuccess) return -static_cast<int>(e);
+        // a partition of a GPU may have no 16 SMs that can form a cluster
+        int clusters = 0;
+        cfg.gridDim = dim3(kPlanCtas);
+        cfg.blockDim = dim3(32 * kPlanWarps);
+        cfg.dynamicSmemBytes = smem;
+        attr[0].val.clusterDim.x = kPlanCtas;
+        cfg.numAttrs = 1;
+        if (cudaOccupancyMaxActiveClusters(&clusters, plan_kernel, &cfg) != cudaSuccess) {
+            cudaGetLastError();
+            clusters = 0;
+        }
+        most_ctas[dev] = clusters > 0 ? kPlanCtas : kPortableCtas;
+    }
+    const PlanShape p = plan_shape(slots, E, most_ctas[dev]);
+    cfg.gridDim = dim3(p.ctas);
+    cfg.blockDim = dim3(32 * p.warps);
+    cfg.dynamicSmemBytes = p.smem;
+    attr[0].val.clusterDim.x = static_cast<unsigned>(p.ctas);
     cfg.numAttrs = 2;
     const cudaError_t e = cudaLaunchKernelEx(&cfg, plan_kernel, ids, slots, E, offsets, order);
     return e == cudaSuccess ? 1 : -static_cast<int>(e);
