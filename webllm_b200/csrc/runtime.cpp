@@ -119,6 +119,24 @@ bool not_capturing(State& s, const char* what) {
     return false;
 }
 
+// The library's device while a launch is made or its errors are read, then the caller's again.
+class OnDevice {
+public:
+    explicit OnDevice(const State& s) {
+        if (cudaGetDevice(&before_) != cudaSuccess) before_ = -1;
+        if (before_ != s.device) err_ = cudaSetDevice(s.device);
+        else before_ = -1;
+    }
+    ~OnDevice() {
+        if (before_ >= 0) cudaSetDevice(before_);
+    }
+    cudaError_t error() const { return err_; }
+
+private:
+    int before_ = -1;
+    cudaError_t err_ = cudaSuccess;
+};
+
 Buffer* find(State& s, int32_t h) {
     auto it = s.live.find(h);
     return it == s.live.end() ? nullptr : &it->second;
@@ -707,6 +725,10 @@ int32_t wllm_sync(void) {
     if (e != cudaSuccess) return cuda_fail(s, e, "wllm_sync");
     e = cudaGetLastError();
     if (e != cudaSuccess) return cuda_fail(s, e, "wllm_sync (pending error)");
+    // the kernels' error words are symbols of the library's device, whatever the
+    // calling thread's is
+    const OnDevice dev(s);
+    if (dev.error() != cudaSuccess) return cuda_fail(s, dev.error(), "wllm_sync");
     const unsigned kerr = wllm::read_and_clear_stream_error() | (wllm::read_and_clear_prefill_error() << 8) |
                           (wllm::read_and_clear_btc_error() << 16) | (wllm::read_and_clear_i8_error() << 24);
     if (kerr)
@@ -1098,24 +1120,6 @@ namespace {
 
 bool float_type(int32_t t) { return t == WLLM_TYPE_F32 || t == WLLM_TYPE_F16 || t == WLLM_TYPE_BF16; }
 int float_bytes(int32_t t) { return t == WLLM_TYPE_F32 ? 4 : 2; }
-
-// The library's device while a launch is made, then the caller's again.
-class OnDevice {
-public:
-    explicit OnDevice(const State& s) {
-        if (cudaGetDevice(&before_) != cudaSuccess) before_ = -1;
-        if (before_ != s.device) err_ = cudaSetDevice(s.device);
-        else before_ = -1;
-    }
-    ~OnDevice() {
-        if (before_ >= 0) cudaSetDevice(before_);
-    }
-    cudaError_t error() const { return err_; }
-
-private:
-    int before_ = -1;
-    cudaError_t err_ = cudaSuccess;
-};
 
 // Byte range of n rows of len elements, stride apart (to the address space's
 // end where it is larger).
