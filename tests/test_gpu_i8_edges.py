@@ -216,3 +216,31 @@ def test_grouped_rows_that_end_inside_a_piece(rt, torch, per_slot, K):
     q.copy_(torch.randint(-127, 128, (rows, K), dtype=torch.int8, device="cuda", generator=g))
     ids = torch.randint(-1, E, (T, k), dtype=torch.int32, device="cuda", generator=g)
     close(torch, grouped(torch, w, ws, q, qs, per_slot, ids, M, K), ref_grouped(torch, w, ws, q, qs, per_slot, ids, K))
+
+
+# ---------------------------------------------------------------- errors
+
+
+def test_a_refused_launch_is_reported_once(rt, torch):
+    """A launch that CUDA refuses (here: into a capture that something else has invalidated) fails its own call; the next
+    wllm_sync does not fail for it too."""
+    from cuda.bindings import runtime as cudart
+
+    logits = torch.randn(2, 8, device="cuda")
+    ids, w = torch.full((2, 2), -9, dtype=torch.int32, device="cuda"), torch.zeros(2, 2, device="cuda")
+    torch.cuda.synchronize()
+    err, st = cudart.cudaStreamCreateWithFlags(cudart.cudaStreamNonBlocking)
+    assert err == cudart.cudaError_t.cudaSuccess
+    (err,) = cudart.cudaStreamBeginCapture(st, cudart.cudaStreamCaptureMode.cudaStreamCaptureModeThreadLocal)
+    assert err == cudart.cudaError_t.cudaSuccess
+    (err,) = cudart.cudaStreamSynchronize(st)  # not allowed in a capture: it is invalid from here on
+    assert err != cudart.cudaError_t.cudaSuccess
+    with pytest.raises(jsep.WllmError, match="wllm_moe_route"):
+        jsep.moe_route(logits.data_ptr(), 8, 2, 8, 2, jsep.MOE_SOFTMAX, True, 1.0, ids.data_ptr(), w.data_ptr(), stream=int(st))
+    cudart.cudaStreamEndCapture(st)
+    cudart.cudaStreamDestroy(st)
+    cudart.cudaGetLastError()
+    rt.jsep_sync()
+    jsep.moe_route(logits.data_ptr(), 8, 2, 8, 2, jsep.MOE_SOFTMAX, True, 1.0, ids.data_ptr(), w.data_ptr(), stream=here(torch))
+    torch.cuda.synchronize()
+    assert torch.equal(ids.long(), logits.topk(2, 1).indices)

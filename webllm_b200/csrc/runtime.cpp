@@ -1133,9 +1133,13 @@ ByteRange rows_range(const void* p, int64_t stride, int64_t n, int64_t len, int 
 
 bool aligned(const void* p, int size) { return (reinterpret_cast<uintptr_t>(p) & (size - 1)) == 0; }
 
-// Counts a launch's kernels or reports its error.
+// Counts a launch's kernels or reports its error, which the runtime then forgets:
+// the next wllm_sync is not to report it once more.
 int32_t launched(State& s, const char* what, int rc) {
-    if (rc < 0) return cuda_fail(s, static_cast<cudaError_t>(-rc), what);
+    if (rc < 0) {
+        cudaGetLastError();
+        return cuda_fail(s, static_cast<cudaError_t>(-rc), what);
+    }
     if (s.capturing) s.captured_kernels += static_cast<uint64_t>(rc);
     else s.counters.kernels_launched += static_cast<uint64_t>(rc);
     return WLLM_STATUS_OK;
