@@ -308,7 +308,7 @@ int32_t wllm_dequantize(int32_t type, const void* src, float* dst, int64_t n, vo
  * calls on several streams are independent and each may be captured into a
  * graph, its first one too. Inputs are not modified; an output may overlap no
  * input of its call (WLLM_STATUS_FAILED where the library can see it). Extents
- * are not checked. N = 0 rows (tokens) is allowed and writes nothing (but
+ * are not checked. K, M, N and n_tokens * n_used are at most 2^31 - 1024. N = 0 rows (tokens) is allowed and writes nothing (but
  * wllm_moe_plan its offsets, all zero). Results do not depend on timing: no sum
  * is taken in an order that varies. */
 

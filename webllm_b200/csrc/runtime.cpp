@@ -1155,7 +1155,8 @@ int32_t wllm_quantize_i8(const wllm_quantize_i8_args* a, void* stream) {
     const char* what = "wllm_quantize_i8";
     if (!a) return fail(s, "%s: null args", what);
     if (!float_type(a->x_type)) return fail(s, "%s: x_type %d is not F32, F16 or BF16", what, a->x_type);
-    if (a->K < 1 || a->N < 0) return fail(s, "%s: K=%d N=%d", what, a->K, a->N);
+    if (a->K < 1 || a->N < 0 || a->K > wllm::kMaxExtent || a->N > wllm::kMaxExtent)
+        return fail(s, "%s: K=%d N=%d (at most 2^31 - 1024)", what, a->K, a->N);
     if (a->glu != 0 && a->glu != WLLM_GLU_SWIGLU && a->glu != WLLM_GLU_GELU)
         return fail(s, "%s: unknown glu kind %d", what, a->glu);
     if (a->glu && a->rms_norm) return fail(s, "%s: glu and rms_norm in one call", what);
@@ -1202,7 +1203,8 @@ int32_t wllm_mul_mat_i8(const wllm_mulmat_i8_args* a, void* stream) {
     const char* what = "wllm_mul_mat_i8";
     if (!a) return fail(s, "%s: null args", what);
     if (!float_type(a->y_type)) return fail(s, "%s: y_type %d is not F32, F16 or BF16", what, a->y_type);
-    if (a->M < 1 || a->K < 1 || a->N < 0) return fail(s, "%s: M=%d K=%d N=%d", what, a->M, a->K, a->N);
+    if (a->M < 1 || a->K < 1 || a->N < 0 || a->M > wllm::kMaxExtent || a->N > wllm::kMaxExtent)
+        return fail(s, "%s: M=%d K=%d N=%d (at most 2^31 - 1024)", what, a->M, a->K, a->N);
     if (a->K > wllm::kMaxK8) return fail(s, "%s: K=%d above %d (the int32 sum)", what, a->K, wllm::kMaxK8);
     if (a->N == 0) return ensure_init(s) ? WLLM_STATUS_OK : WLLM_STATUS_FAILED;
     const int size = float_bytes(a->y_type);
@@ -1241,7 +1243,7 @@ int32_t wllm_mul_mat_i8(const wllm_mulmat_i8_args* a, void* stream) {
 static int32_t moe_sizes(State& s, const char* what, int32_t T, int32_t k, int32_t E) {
     if (T < 0 || k < 1 || k > wllm::kMaxUsed || E < 1 || E > wllm::kMaxExperts)
         return fail(s, "%s: n_tokens=%d n_used=%d (1..%d) n_expert=%d (1..%d)", what, T, k, wllm::kMaxUsed, E, wllm::kMaxExperts);
-    if (static_cast<int64_t>(T) * k > 0x7fffffffLL) return fail(s, "%s: n_tokens * n_used exceeds 2^31", what);
+    if (static_cast<int64_t>(T) * k > wllm::kMaxExtent) return fail(s, "%s: n_tokens * n_used exceeds 2^31 - 1024", what);
     return WLLM_STATUS_OK;
 }
 
@@ -1294,7 +1296,7 @@ int32_t wllm_mul_mat_id_i8(const wllm_mulmat_id_i8_args* a, void* stream) {
     if (!float_type(a->y_type)) return fail(s, "%s: y_type %d is not F32, F16 or BF16", what, a->y_type);
     if (a->reserved != 0) return fail(s, "%s: reserved must be 0", what);
     if (const int32_t rc = moe_sizes(s, what, a->n_tokens, a->n_used, a->n_expert)) return rc;
-    if (a->M < 1 || a->K < 1) return fail(s, "%s: M=%d K=%d", what, a->M, a->K);
+    if (a->M < 1 || a->K < 1 || a->M > wllm::kMaxExtent) return fail(s, "%s: M=%d K=%d (at most 2^31 - 1024)", what, a->M, a->K);
     if (a->K > wllm::kMaxK8) return fail(s, "%s: K=%d above %d (the int32 sum)", what, a->K, wllm::kMaxK8);
     if (a->n_tokens == 0) return ensure_init(s) ? WLLM_STATUS_OK : WLLM_STATUS_FAILED;
     const int size = float_bytes(a->y_type);
@@ -1347,7 +1349,7 @@ int32_t wllm_moe_combine(int32_t z_type, const void* z, int64_t z_stride, const 
     const char* what = "wllm_moe_combine";
     if (!float_type(z_type) || !float_type(y_type)) return fail(s, "%s: types %d, %d are not F32, F16 or BF16", what, z_type, y_type);
     if (const int32_t rc = moe_sizes(s, what, T, k, 1)) return rc;
-    if (M < 1) return fail(s, "%s: M=%d", what, M);
+    if (M < 1 || M > wllm::kMaxExtent) return fail(s, "%s: M=%d (at most 2^31 - 1024)", what, M);
     if (T == 0) return ensure_init(s) ? WLLM_STATUS_OK : WLLM_STATUS_FAILED;
     if (!z || !weights || !y) return fail(s, "%s: null pointer", what);
     const int zs = float_bytes(z_type), ys = float_bytes(y_type);

@@ -193,6 +193,9 @@ struct MulMatI8 {
     int32_t E, k;
     int32_t per_slot, y_type;
 };
+// Rows, channels and values of a row: the kernels' 32-bit indices go past the last
+// by less than what is left to 2^31.
+constexpr int kMaxExtent = 0x7fffffff - 1023;
 constexpr int kMaxK8 = 131071;  // |sum| <= K * 128 * 128 < 2^31
 int launch_mul_mat_i8(const MulMatI8& o, cudaStream_t stream, int num_sms);
 int launch_mul_mat_id_i8(const MulMatI8& o, cudaStream_t stream, int num_sms);
