@@ -5,11 +5,11 @@ from __future__ import annotations
 import os
 import subprocess
 import sys
-
 import zlib
 
 import pytest
 
+from test_i8_plan import GROUPS, PRODUCTS
 from webllm_b200 import jsep
 
 pytestmark = pytest.mark.gpu
@@ -244,3 +244,155 @@ def test_a_refused_launch_is_reported_once(rt, torch):
     jsep.moe_route(logits.data_ptr(), 8, 2, 8, 2, jsep.MOE_SOFTMAX, True, 1.0, ids.data_ptr(), w.data_ptr(), stream=here(torch))
     torch.cuda.synchronize()
     assert torch.equal(ids.long(), logits.topk(2, 1).indices)
+
+
+# ---------------------------------------------------------------- every form of the products' kernel
+
+
+def product(torch, w, ws, q, qs, M, K, N, t="float32"):
+    y = torch.full((N, M), float("nan"), dtype=getattr(torch, t), device="cuda")
+    jsep.mul_mat_i8(w.data_ptr(), w.stride(0), ws.data_ptr(), q.data_ptr(), q.stride(0), qs.data_ptr(), {"float32": 0, "float16": 1, "bfloat16": 30}[t],
+                    y.data_ptr(), M, M, K, N, stream=here(torch))
+    torch.cuda.synchronize()
+    return y
+
+
+def rows8(torch, g, *shape):
+    """int8 rows of the last of `shape` values, padded to 16 bytes with values of their own, and scales."""
+    q = torch.randint(-127, 128, (*shape[:-1], up16(shape[-1])), dtype=torch.int8, device="cuda", generator=g)
+    return q, torch.rand(shape[:-1], device="cuda", generator=g) * 0.01 + 1e-3
+
+
+@pytest.mark.parametrize("i", range(len(PRODUCTS)))
+def test_product_of_every_mode(rt, torch, i):
+    M, K, N = PRODUCTS[i][3:]
+    g = gen_of(torch, "mode", i)
+    (w, ws), (q, qs) = rows8(torch, g, M, K), rows8(torch, g, N, K)
+    ref = (q[:, :K].double() @ w[:, :K].double().t()) * qs.double()[:, None] * ws.double()
+    for t in ("float32", "float16", "bfloat16"):
+        close(torch, product(torch, w, ws, q, qs, M, K, N, t), ref)
+
+
+@pytest.mark.parametrize("how", ["even", "skewed", "holes"])
+@pytest.mark.parametrize("i", range(len(GROUPS)))
+def test_grouped_of_every_mode(rt, torch, i, how):
+    """Routings that the plan, which counts on an even one, does not expect among them: most slots on one expert, and slots
+    and experts without one another."""
+    M, K, E, T, k = GROUPS[i][3:]
+    g = gen_of(torch, "grouped mode", i, how)
+    per_slot = bool(i & 1)
+    (w, ws), (q, qs) = rows8(torch, g, E, M, K), rows8(torch, g, T * k if per_slot else T, K)
+    if how == "even":
+        ids = torch.rand(T, E, device="cuda", generator=g).argsort(1)[:, :k].to(torch.int32).contiguous()
+    elif how == "skewed":
+        ids = torch.where(torch.rand(T, k, device="cuda", generator=g) < 0.9, E - 1, 0).to(torch.int32)
+    else:
+        ids = torch.randint(-3, E + 2, (T, k), dtype=torch.int32, device="cuda", generator=g)
+        ids[ids == E // 2] = -1
+    ref = ref_grouped(torch, w, ws, q, qs, per_slot, ids, K)
+    for t in ("float32", "bfloat16"):
+        close(torch, grouped(torch, w, ws, q, qs, per_slot, ids, M, K, t), ref)
+
+
+@pytest.mark.parametrize("how", ["even", "skewed", "holes", "none"])
+@pytest.mark.parametrize("E", [575, 576, 577, 1000, 1024])
+def test_grouped_of_many_experts(rt, torch, E, how):
+    """More experts than the kernel has threads: its running sum over their tiles takes a second step."""
+    M, K, T, k = 140, 200, 300, 5
+    g = gen_of(torch, "many experts", E, how)
+    (w, ws), (q, qs) = rows8(torch, g, E, M, K), rows8(torch, g, T, K)
+    if how == "even":
+        ids = torch.rand(T, E, device="cuda", generator=g).argsort(1)[:, :k].to(torch.int32).contiguous()
+    elif how == "skewed":  # the last experts
+        ids = (E - 1 - torch.randint(0, 4, (T, k), device="cuda", generator=g) ** 2).to(torch.int32)
+    elif how == "holes":
+        ids = torch.randint(-E, E, (T, k), dtype=torch.int32, device="cuda", generator=g)
+    else:
+        ids = torch.full((T, k), E, dtype=torch.int32, device="cuda")
+    close(torch, grouped(torch, w, ws, q, qs, False, ids, M, K), ref_grouped(torch, w, ws, q, qs, False, ids, K))
+
+
+# ---------------------------------------------------------------- far offsets
+
+
+def test_grouped_weights_past_32_bits(rt, torch):
+    """Experts whose weights begin past 2^32 bytes."""
+    E, M, K, T, k = 140, 4096, 8192, 9, 3
+    g = gen_of(torch, "far experts")
+    (w, ws), (q, qs) = rows8(torch, g, E, M, K), rows8(torch, g, T, K)
+    ids = torch.tensor([E - 1, E - 2, 0], dtype=torch.int32, device="cuda").repeat(T, 1)
+    close(torch, grouped(torch, w, ws, q, qs, False, ids, M, K), ref_grouped(torch, w, ws, q, qs, False, ids, K))
+
+
+def test_rows_past_2_31_elements(rt, torch):
+    """Outputs of a dense and a grouped product, inputs of the quantiser and of the weighted sum whose last rows lie past
+    2^31 elements (f16, so past 2^32 bytes too)."""
+    N, M, K = 66000, 33000, 32
+    g = gen_of(torch, "far rows")
+    (w, ws), (q, qs) = rows8(torch, g, 2, M, K), rows8(torch, g, N, K)
+    some = torch.cat([torch.arange(0, 3), torch.arange(N // 2, N // 2 + 3), torch.arange(N - 40, N)]).cuda()
+
+    def ref(e):
+        return (q[some, :K].double() @ w[e, :, :K].double().t()) * qs[some].double()[:, None] * ws[e].double()
+
+    y = product(torch, w[0], ws[0], q, qs, M, K, N, "float16")
+    close(torch, y[some], ref(0))
+    ids = torch.ones(N, 1, dtype=torch.int32, device="cuda")
+    del y
+    y = grouped(torch, w, ws, q, qs, False, ids, M, K, "float16")
+    close(torch, y[some], ref(1))
+    # rows of y in pairs, weighted
+    T, weights = N // 2, torch.rand(N // 2, 2, device="cuda", generator=g)
+    z = torch.full((T, M), float("nan"), device="cuda")
+    jsep.moe_combine(jsep.GGML_TYPE_F16, y.data_ptr(), M, weights.data_ptr(), 0, z.data_ptr(), M, T, 2, M, stream=here(torch))
+    torch.cuda.synchronize()
+    parts = y.view(T, 2, M)[-40:].double() * weights[-40:, :, None].double()
+    off = (z[-40:].double() - parts.sum(1)).abs()
+    assert (off <= 3 * U32 * parts.abs().sum(1)).all()  # two products and a sum
+    del z, parts, off
+    q8, s = quantize(torch, y)
+    v = y[some].double()
+    rs = (v.abs().amax(1) / 127).float()
+    assert torch.equal(s[some], rs)
+    assert torch.equal(q8[some], (v / rs.double()[:, None]).round().clamp(-127, 127).to(torch.int8))
+
+
+# ---------------------------------------------------------------- rows that are not ordinary, in every form of the quantiser
+
+
+@pytest.mark.parametrize("t", ["float32", "float16", "bfloat16"])
+@pytest.mark.parametrize("kind", [0, jsep.GLU_SWIGLU, jsep.GLU_GELU])
+@pytest.mark.parametrize("N,K", [(13, 100), (13, 20003), (613, 100), (613, 1999)])
+def test_quantize_rows_that_are_not_ordinary(rt, torch, t, kind, N, K):
+    """NaN, infinities, zero, the smallest and the largest numbers in rows of their own among ordinary rows: a CTA and a warp
+    a row, in whole vectors and behind them. The others come out as they do without."""
+    g = gen_of(torch, "not ordinary", t, kind, N, K)
+    dt = getattr(torch, t)
+    top, low = torch.finfo(dt).max, torch.finfo(dt).tiny
+    x = torch.randn(N, K, device="cuda", generator=g).to(dt)
+    up = torch.randn(N, K, device="cuda", generator=g).to(dt)
+    kw = dict(glu=kind, up_ptr=up.data_ptr(), up_stride=K) if kind else {}
+    alone = quantize(torch, x, **kw)
+    bad = {1: (0, float("nan")), 2: (K - 1, float("nan")), 3: (K // 2, float("inf")), 4: (K - 1, float("inf"))}
+    for r, (k, v) in bad.items():
+        x[r, k] = v
+    x[5] = 0
+    x[6] = -0.0
+    x[7] = top
+    x[8], up[8] = low, 1
+    x[9], up[9] = 1, low
+    if kind:
+        up[10, K - 2] = float("nan")
+        bad[10] = None
+    q, s = quantize(torch, x, **kw)
+    for r in bad:
+        assert torch.isnan(s[r]) and (q[r] == 0).all(), r
+    assert (s[5:7] == 0).all() and (q[5:7] == 0).all()
+    rest = [n for n in range(N) if n not in (1, 2, 3, 4, 5, 6, 7, 8, 9, 10)]
+    assert torch.equal(q[rest], alone[0][rest]) and torch.equal(s[rest], alone[1][rest])
+    if not kind:
+        for r in (7, 8, 9, 10):
+            v = x[r].double()
+            rs = (v.abs().amax() / 127).float()
+            assert torch.equal(s[r], rs)
+            assert torch.equal(q[r], (v / rs.double()).round().clamp(-127, 127).to(torch.int8))
