@@ -104,10 +104,11 @@ __device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, unsign
     return false;
 }
 // Bounded wait whatever the poison flag says, for what is in flight at exit.
-__device__ __forceinline__ void mbar_drain(uint64_t* bar, uint32_t parity) {
+__device__ __forceinline__ bool mbar_drain(uint64_t* bar, uint32_t parity) {
     for (uint32_t i = 0; i < kSpinLimit; ++i)
-        if (mbar_try(bar, parity)) return;
+        if (mbar_try(bar, parity)) return true;
     atomicOr(&g_i8_error, 8u);
+    return false;
 }
 __device__ __forceinline__ void mbar_arrive(uint64_t* bar) {
     asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
@@ -244,6 +245,11 @@ __device__ __forceinline__ void cluster_sync() {
 // The same without ordering memory (global stores before it are not waited for).
 __device__ __forceinline__ void cluster_meet() {
     asm volatile("barrier.cluster.arrive.relaxed.aligned;\n\tbarrier.cluster.wait.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void st_cluster(uint32_t local, uint32_t rank, int v) {
+    uint32_t remote;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(local), "r"(rank));
+    asm volatile("st.shared::cluster.s32 [%0], %1;" ::"r"(remote), "r"(v) : "memory");
 }
 __device__ __forceinline__ int4 ld_cluster4(uint32_t local, uint32_t rank) {
     uint32_t remote;
@@ -535,11 +541,12 @@ __global__ void __launch_bounds__(GROUPED ? kThreads + 2 * kLoaders : kThreads, 
                     ring.next();
                 }
             }
-            if (*poisoned && (!PAIR || rank == 0)) {  // the copies in flight land before the CTA ends
-                for (int p = 0; p < filled; ++p) {
-                    ring.s = ring.s ? ring.s - 1 : (ring.parity ^= 1, stages - 1);
-                    mbar_drain(&full[ring.s], ring.parity);
-                }
+            // The copies in flight land before the CTA ends. (Nothing else is left to do
+            // here; where all went well the MMAs wait for the same.) Those of a pair's
+            // second CTA are signalled to the first, but their stages are freed here.
+            for (int p = 0; p < filled; ++p) {
+                ring.s = ring.s ? ring.s - 1 : (ring.parity ^= 1, stages - 1);
+                if (!mbar_drain(PAIR && rank ? &empty[ring.s] : &full[ring.s], ring.parity)) break;
             }
         }
     } else if (warp == 1) {
@@ -578,11 +585,12 @@ __global__ void __launch_bounds__(GROUPED ? kThreads + 2 * kLoaders : kThreads, 
                     last = &empty[s], last_parity = ring.parity;
                     ring.next();
                 }
+                if (!ok) break;  // an accumulator that is not whole is not handed over
                 if constexpr (PAIR) umma_commit_pair(&acc_full[buf]);
                 else umma_commit(&acc_full[buf]);
             }
-            // MMAs still in flight (only after a time-out) end before the TMEM is freed
-            if (*poisoned && last) mbar_drain(last, last_parity);
+            // MMAs in flight end before the TMEM is freed
+            if (last) mbar_drain(last, last_parity);
         }
     } else if (warp < 2 + kEpiWarps) {
         // ---------------- epilogue ----------------
@@ -729,7 +737,10 @@ __global__ void __launch_bounds__(GROUPED ? kThreads + 2 * kLoaders : kThreads, 
         if (untold >= 0) tell(untold);
     }
     if constexpr (SPLIT) {
-        // one item per cluster, so that the sum over the splits comes after all roles
+        // one item per cluster, so that the sum over the splits comes after all roles;
+        // a tile that one CTA gave up on is summed by none
+        if (*poisoned)
+            for (int r = 0; r < P.splits; ++r) st_cluster(smem_u32(&poison), r, 1);
         __syncwarp();
         cluster_sync();
         if (item0 < items && !*poisoned) {
