@@ -619,6 +619,7 @@ __global__ void __launch_bounds__(GROUPED ? kThreads + 2 * kLoaders : kThreads, 
             next_scale = fetch_scale(next_row);
         }
         uint32_t t = 0;
+        bool ok = true;
         for (int i = item0; i < items; i += item_step, ++t) {
             const Item it = next;
             const uint32_t buf = t & 1;
@@ -636,8 +637,9 @@ __global__ void __launch_bounds__(GROUPED ? kThreads + 2 * kLoaders : kThreads, 
             }
             asm volatile("bar.sync 1, %0;" ::"n"(32 * kEpiWarps) : "memory");  // the epilogue warps
             // after a time-out the items are still walked (the epilogue's warps meet at
-            // the barrier above), without their stores
-            const bool ok = mbar_wait(&acc_full[buf], (t >> 1) & 1, 2u, poisoned);
+            // the barrier above), without their stores and without handing accumulators
+            // back; a warp's lanes, which read the TMEM together, give up together
+            ok = __all_sync(0xffffffffu, ok && mbar_wait(&acc_full[buf], (t >> 1) & 1, 2u, poisoned));
             tc_fence_after();
             if (more) next_scale = fetch_scale(next_row);
             const uint32_t d = tmem + buf * P.tile_n + (static_cast<uint32_t>(32 * quad) << 16);
@@ -660,7 +662,7 @@ __global__ void __launch_bounds__(GROUPED ? kThreads + 2 * kLoaders : kThreads, 
             }
             tc_fence_before();
             __syncwarp();
-            if (lane == 0) {
+            if (ok && lane == 0) {
                 if constexpr (PAIR) mbar_arrive_at(&acc_free[buf], 0);
                 else mbar_arrive(&acc_free[buf]);
             }
