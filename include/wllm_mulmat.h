@@ -247,13 +247,17 @@ int32_t wllm_mul_mat_batch_tp(const wllm_mulmat_args* ops, const wllm_tp_outputs
 int32_t wllm_tp_wait(const wllm_tp_group* group, void* stream);
 
 /* How many polls a bounded device-side wait of the decode kernels (pipeline
- * barriers, a peer rank's signal) makes before it gives up, for launches
- * enqueued after this call; 0 restores the default of 2^26 polls (seconds).
+ * barriers, a peer rank's signal) and of the 8-bit products (pipeline barriers)
+ * makes before it gives up, for launches enqueued after this call; 0 restores
+ * the defaults, 2^26 polls of the decode kernels and 2^20 of the 8-bit products.
+ * A poll of a peer's signal takes well under a microsecond, one of a pipeline
+ * barrier up to 4.
  * A wait that gives up records an error code, the kernel still ends, and the
  * next wllm_sync returns WLLM_STATUS_FAILED with the code in its message: a
- * dead or stalled peer rank surfaces as an error rather than a hang. A small
- * limit can fail healthy but slow launches. No counterpart in the reference
- * (one browser GPU, no device-side waits). */
+ * dead or stalled peer rank surfaces as an error rather than a hang. What the
+ * launch writes is not to be used then. A small limit can fail healthy but slow
+ * launches. No counterpart in the reference (one browser GPU, no device-side
+ * waits). */
 int32_t wllm_set_wait_limit(uint32_t polls);
 
 /* The library's CUDA stream (a cudaStream_t), so a host can order its own
@@ -308,7 +312,11 @@ int32_t wllm_dequantize(int32_t type, const void* src, float* dst, int64_t n, vo
  * calls on several streams are independent and each may be captured into a
  * graph, its first one too. Inputs are not modified; an output may overlap no
  * input of its call (WLLM_STATUS_FAILED where the library can see it). Extents
- * are not checked. K, M, N and n_tokens * n_used are at most 2^31 - 1024. N = 0 rows (tokens) is allowed and writes nothing (but
+ * are not checked. K, M, N and n_tokens * n_used are at most 2^31 - 1024. A
+ * device-side wait of the products that gave up (wllm_set_wait_limit) is told by
+ * the first wllm_sync after the launch has ended; that waits for the library's
+ * stream alone, so a caller that launches on a stream of its own synchronises
+ * with it first. N = 0 rows (tokens) is allowed and writes nothing (but
  * wllm_moe_plan its offsets, all zero). Results do not depend on timing: no sum
  * is taken in an order that varies. */
 

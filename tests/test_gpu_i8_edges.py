@@ -9,7 +9,7 @@ import zlib
 
 import pytest
 
-from test_i8_plan import GROUPS, PRODUCTS
+from test_i8_plan import GROUPS, LONG, PRODUCTS
 from webllm_b200 import jsep
 
 pytestmark = pytest.mark.gpu
@@ -396,3 +396,45 @@ def test_quantize_rows_that_are_not_ordinary(rt, torch, t, kind, N, K):
             rs = (v.abs().amax() / 127).float()
             assert torch.equal(s[r], rs)
             assert torch.equal(q[r], (v / rs.double()).round().clamp(-127, 127).to(torch.int8))
+
+
+# ---------------------------------------------------------------- waits that give up
+
+
+@pytest.mark.parametrize("i", range(len(LONG)))
+def test_a_wait_that_gives_up_is_reported(rt, torch, i):
+    """With a limit of one poll (4 us) the epilogue of a long K, whose MMAs take 10 us and more, gives up, in every mode: the
+    launch ends, the next wllm_sync says so, nothing is stored, and with the limit restored the same call gives what it gave
+    before. Nothing stalls here: what the epilogue would not wait for is on its way, and the kernel ends after it."""
+    M, K, E, N = LONG[i][2:]  # E = 0: dense
+    g = gen_of(torch, "waits", i)
+    (w, ws), (q, qs) = rows8(torch, g, max(E, 1), M, K), rows8(torch, g, N, K)
+    offsets = (torch.arange(E + 1, device="cuda") * (N // max(E, 1))).to(torch.int32)
+    order = torch.arange(N, dtype=torch.int32, device="cuda")
+    y = torch.full((N, M), float("nan"), device="cuda")
+    torch.cuda.synchronize()
+
+    def call():  # on the library's stream, which wllm_sync waits for
+        if E:
+            jsep.mul_mat_id_i8(w.data_ptr(), w.stride(1), w.stride(0), ws.data_ptr(), q.data_ptr(), q.stride(0), qs.data_ptr(), False, offsets.data_ptr(),
+                               order.data_ptr(), 0, y.data_ptr(), M, M, K, E, N, 1)
+        else:
+            jsep.mul_mat_i8(w.data_ptr(), w.stride(1), ws.data_ptr(), q.data_ptr(), q.stride(0), qs.data_ptr(), 0, y.data_ptr(), M, M, K, N)
+        return jsep.load_library().wllm_sync()
+
+    assert call() == jsep.STATUS_OK
+    before = y.clone()
+    assert not torch.isnan(before).any()
+    y.fill_(float("nan"))
+    torch.cuda.synchronize()
+    try:
+        jsep.set_wait_limit(1)
+        rc = call()
+    finally:
+        jsep.set_wait_limit(0)
+    msg = jsep.last_error()
+    assert rc == jsep.STATUS_FAILED and "gave up waiting" in msg and "8-bit" in msg, msg
+    assert int(msg.split("code 0x")[1].split(":")[0], 16) >> 24 & 2, msg  # an accumulator
+    assert torch.isnan(y).all()
+    assert call() == jsep.STATUS_OK
+    assert torch.equal(y, before)

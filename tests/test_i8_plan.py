@@ -129,6 +129,14 @@ GROUPS = [
     (PAIR_SHORT, 1, 128, 270, 144, 3, 501, 3),
 ]
 
+# Of every mode one whose items' MMAs take 10 us and more, one or two items a CTA: mode, splits, M, K, E (0: dense), tokens.
+LONG = [
+    (SINGLE, 1, 17920, 65536, 0, 16), (SPLIT, 8, 128, 131056, 0, 1), (SPLIT, 8, 256, 131056, 0, 256),
+    (PAIR, 1, 17920, 16384, 0, 256), (PAIR_SHORT, 1, 17920, 32768, 0, 64),
+    (SINGLE, 1, 128, 16384, 200, 200), (SPLIT, 8, 128, 131056, 1, 3), (PAIR, 1, 17920, 16384, 1, 256),
+    (PAIR_SHORT, 1, 17920, 32768, 1, 64),
+]
+
 
 def test_products_of_every_mode(host):
     """The sizes that the GPU tests run, so that each of the kernel's forms is reached."""
@@ -138,3 +146,6 @@ def test_products_of_every_mode(host):
         assert grouped_plan(host, M, K, E, T * k)[:3] == (form[0], form[2], form[1])
     every = {(SINGLE, 1), (SPLIT, 2), (SPLIT, 4), (SPLIT, 8), (PAIR, 1), (PAIR_SHORT, 1)}
     assert {(c[0], c[1]) for c in PRODUCTS} == every and {(c[0], c[1]) for c in GROUPS} == every
+    for mode, splits, M, K, E, N in LONG:
+        plan = grouped_plan(host, M, K, E, N) if E else product_plan(host, M, K, N)
+        assert (plan[0], plan[2]) == (mode, splits)

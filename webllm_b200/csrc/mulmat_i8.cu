@@ -43,15 +43,16 @@
 // pipe above (4096 x 14336 -> 4096: 160 us, 3.0 POP/s; in a long run the power
 // limit, 2.5 to 2.8).
 //
-// Every mbarrier wait is bounded: on time-out the CTA records an error code
-// (read by wllm_sync), stops issuing, waits for its copies and MMAs in flight
-// and frees its TMEM.
+// Every mbarrier wait is bounded (wllm_set_wait_limit): on time-out the CTA records
+// an error code (read by wllm_sync), stops issuing, waits for its copies and MMAs
+// in flight and frees its TMEM.
 #include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <stdint.h>
 
 #include <algorithm>
+#include <atomic>
 
 #include "i8_plan.h"
 #include "wllm_internal.h"
@@ -67,7 +68,7 @@ constexpr int kThreads = 64 + 32 * kEpiWarps;  // copies, MMAs, epilogue
 constexpr int kLoaders = 128;       // threads that gather a stage's tokens; there are two such groups
 constexpr int kMaxStages = 12;
 constexpr int kSmemBytes = 208 * 1024;  // dynamic, beside up to 17 KB of tables and barriers
-constexpr uint32_t kSpinLimit = 1u << 26;
+constexpr uint32_t kSpinLimit = 1u << 20;  // polls of a barrier, each of which the hardware ends after 4 us: some 4 s
 
 struct I8Args {
     CUtensorMap wmap;  // weights: [E][M][K] bytes, box 128 x 128 x 1
@@ -76,6 +77,7 @@ struct I8Args {
     int32_t tile_n;    // tokens of a full tile, a multiple of 16 (pair: of 32)
     int32_t tiles_m, tiles_n, chunks, stages, splits;  // tiles_n: dense; chunks: of a stage's bytes of K
     int32_t tmem_cols;
+    uint32_t spin_limit;  // polls before a wait gives up
 };
 
 __device__ __forceinline__ uint32_t smem_u32(const void* p) { return static_cast<uint32_t>(__cvta_generic_to_shared(p)); }
@@ -94,8 +96,8 @@ __device__ __forceinline__ bool mbar_try(uint64_t* bar, uint32_t parity) {
     return ok != 0;
 }
 // Bounded wait; a time-out poisons the CTA (every later wait returns at once).
-__device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, unsigned code, volatile int* poisoned) {
-    for (uint32_t i = 0; i < kSpinLimit; ++i) {
+__device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, unsigned code, volatile int* poisoned, uint32_t limit) {
+    for (uint32_t i = 0; i < limit; ++i) {
         if (mbar_try(bar, parity)) return true;
         if ((i & 255u) == 255u && *poisoned) return false;
     }
@@ -517,7 +519,7 @@ __global__ void __launch_bounds__(GROUPED ? kThreads + 2 * kLoaders : kThreads, 
                 const int cols = (it.rows + 31) & ~31, n0 = it.first + (PAIR ? rank * (cols / 2) : 0);
                 for (int c = c0; c < c1; ++c) {
                     const int s = ring.s;
-                    ok = filled < stages || mbar_wait(&empty[s], ring.parity ^ 1, 1u, poisoned);
+                    ok = filled < stages || mbar_wait(&empty[s], ring.parity ^ 1, 1u, poisoned, P.spin_limit);
                     if (!ok) break;
                     const uint32_t a = smem_u32(smem + s * stage_bytes);
                     const uint32_t b = a + kSub * kABytes;
@@ -561,12 +563,12 @@ __global__ void __launch_bounds__(GROUPED ? kThreads + 2 * kLoaders : kThreads, 
                 const Item it = walk.at(i);
                 const uint32_t idesc = PAIR ? i8_idesc(2 * kTileM, (it.rows + 31) & ~31) : i8_idesc(kTileM, (it.rows + 15) & ~15);
                 const uint32_t buf = t & 1, d = tmem + buf * P.tile_n;
-                ok = t < 2 || mbar_wait(&acc_free[buf], ((t >> 1) - 1) & 1, 2u, poisoned);
+                ok = t < 2 || mbar_wait(&acc_free[buf], ((t >> 1) - 1) & 1, 2u, poisoned, P.spin_limit);
                 if (!ok) break;
                 tc_fence_after();
                 for (int c = c0; c < c1; ++c) {
                     const int s = ring.s;
-                    ok = mbar_wait(&full[s], ring.parity, 4u, poisoned);
+                    ok = mbar_wait(&full[s], ring.parity, 4u, poisoned, P.spin_limit);
                     if (!ok) break;
                     tc_fence_after();
                     const uint32_t a = smem_u32(smem + s * stage_bytes);
@@ -639,7 +641,7 @@ __global__ void __launch_bounds__(GROUPED ? kThreads + 2 * kLoaders : kThreads, 
             // after a time-out the items are still walked (the epilogue's warps meet at
             // the barrier above), without their stores and without handing accumulators
             // back; a warp's lanes, which read the TMEM together, give up together
-            ok = __all_sync(0xffffffffu, ok && mbar_wait(&acc_full[buf], (t >> 1) & 1, 2u, poisoned));
+            ok = __all_sync(0xffffffffu, ok && mbar_wait(&acc_full[buf], (t >> 1) & 1, 2u, poisoned, P.spin_limit));
             tc_fence_after();
             if (more) next_scale = fetch_scale(next_row);
             const uint32_t d = tmem + buf * P.tile_n + (static_cast<uint32_t>(32 * quad) << 16);
@@ -712,7 +714,7 @@ __global__ void __launch_bounds__(GROUPED ? kThreads + 2 * kLoaders : kThreads, 
             for (int c = c0; c < c1; ++c, ++q, ring.next()) {
                 if ((q & 1) != mine) continue;
                 const int s = ring.s;
-                ok = q < stages || mbar_wait(&empty[s], ring.parity ^ 1, 1u, poisoned);
+                ok = q < stages || mbar_wait(&empty[s], ring.parity ^ 1, 1u, poisoned, P.spin_limit);
                 ok = __all_sync(0xffffffffu, ok);
                 if (!ok) break;
                 // piece p of row r lies at r * 128 + (p ^ (r % 8)) * 16; of the last piece only
@@ -856,6 +858,8 @@ int launch_general(const MulMatI8& o, cudaStream_t stream, int num_sms) {
     return e == cudaSuccess ? 1 : -static_cast<int>(e);
 }
 
+std::atomic<uint32_t> g_i8_wait_limit{kSpinLimit};
+
 template <bool GROUPED>
 int launch(const MulMatI8& o, cudaStream_t stream, int num_sms) {
     const uintptr_t bits = reinterpret_cast<uintptr_t>(o.w) | reinterpret_cast<uintptr_t>(o.q) |
@@ -872,6 +876,7 @@ int launch(const MulMatI8& o, cudaStream_t stream, int num_sms) {
     P.o = o;
     P.tile_n = plan.tile_n;
     P.splits = plan.splits;
+    P.spin_limit = g_i8_wait_limit.load();
     const bool pair = is_pair(plan.mode);
     const int tile_m = pair ? 2 * kTileM : kTileM, sub = chunks_of_stage(plan.mode);
     P.tiles_m = (o.M + tile_m - 1) / tile_m;
@@ -934,6 +939,8 @@ int launch_mul_mat_id_i8(const MulMatI8& o, cudaStream_t stream, int num_sms) {
     g_i8_launched = true;
     return launch<true>(o, stream, num_sms);
 }
+
+void set_i8_wait_limit(uint32_t polls) { g_i8_wait_limit.store(polls ? polls : kSpinLimit); }
 
 unsigned read_and_clear_i8_error() {
     if (!g_i8_launched) return 0;

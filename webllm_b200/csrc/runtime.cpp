@@ -744,6 +744,7 @@ int32_t wllm_set_wait_limit(uint32_t polls) {
     State& s = S();
     std::lock_guard<std::mutex> g(s.mu);
     wllm::set_stream_wait_limit(polls);
+    wllm::set_i8_wait_limit(polls);
     return WLLM_STATUS_OK;
 }
 

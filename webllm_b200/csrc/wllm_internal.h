@@ -200,6 +200,7 @@ constexpr int kMaxK8 = 131071;  // |sum| <= K * 128 * 128 < 2^31
 int launch_mul_mat_i8(const MulMatI8& o, cudaStream_t stream, int num_sms);
 int launch_mul_mat_id_i8(const MulMatI8& o, cudaStream_t stream, int num_sms);
 unsigned read_and_clear_i8_error();
+void set_i8_wait_limit(uint32_t polls);  // 0: the default
 
 // Top-k router, slots by expert, weighted sum over a token's slots (moe.cu).
 constexpr int kMaxExperts = 1024;

@@ -547,8 +547,8 @@ def tp_wait(group: TpGroup, stream: int = 0) -> int:
 
 
 def set_wait_limit(polls: int) -> None:
-    """Polls before a device-side wait of the decode kernels gives up (0: the
-    default); a wait that gives up fails the next sync instead of hanging."""
+    """Polls before a device-side wait of the decode kernels or of the 8-bit
+    products gives up (0: the defaults); a wait that gives up fails the next sync instead of hanging."""
     _check(load_library().wllm_set_wait_limit(int(polls)), "wllm_set_wait_limit")
 
 
