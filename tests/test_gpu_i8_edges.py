@@ -166,6 +166,30 @@ def test_swiglu_of_gates_far_below_zero(rt, torch, t, off, N, K):
     assert ((q.double() * sd[:, None] - v).abs() <= 0.5 * sd[:, None] + eps * v.abs() + 127 * sd[:, None] * 2 * U32 + (127 + 6) * sub).all()
 
 
+# ---------------------------------------------------------------- router
+
+
+@pytest.mark.parametrize("E,k", [(8, 3), (60, 8), (1024, 32)])
+@pytest.mark.parametrize("normalize", [False, True])
+def test_sigmoid_of_logits_far_below_zero(rt, torch, E, k, normalize):
+    """Rows of logits about -60, -70, .. -103, where a sigmoid is e^l and, from -87 on, below f32's normals: the weights by the
+    64-bit formula. e^l and e^(l - top) by expf (2 ulp = 4 u, their arguments off by at most u 104), a sum of at most 32 terms
+    (5 steps), a quotient and a product, and half a subnormal step (2^-150) where the weight itself is so small; a
+    normalised one's terms are e^(l - top), whose rounding is relative to 1."""
+    g = gen_of(torch, "sigmoid", E, k)
+    base = torch.tensor([-60.0, -63.9, -64.1, -70, -85, -87, -88, -89, -90, -95, -100, -101], device="cuda")[:, None]
+    l = base - 2 * torch.rand(len(base), E, device="cuda", generator=g)
+    ids, w = torch.empty(len(base), k, dtype=torch.int32, device="cuda"), torch.empty(len(base), k, device="cuda")
+    jsep.moe_route(l.data_ptr(), E, len(base), E, k, jsep.MOE_SIGMOID, normalize, 1.0, ids.data_ptr(), w.data_ptr(), stream=here(torch))
+    torch.cuda.synchronize()
+    best = l.sort(dim=1, descending=True, stable=True)
+    assert torch.equal(ids.long(), best.indices[:, :k])
+    p = 1 / (1 + (-best.values[:, :k].double()).exp())
+    ref = p / p.sum(1, keepdim=True) if normalize else p
+    tol = (4 + 104 + 5 + 4 + 2) * U32 * ref * (2 if normalize else 1) + 2.0 ** -150
+    assert ((w.double() - ref).abs() <= tol).all()
+
+
 # ---------------------------------------------------------------- grouped product
 
 

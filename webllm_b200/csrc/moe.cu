@@ -79,10 +79,14 @@ __global__ void __launch_bounds__(32 * kRouteWarps) route_kernel(const MoeRoute 
     }
     auto value = [](uint32_t k) { return __uint_as_float((k & 0x80000000u) ? (k & 0x7fffffffu) : ~k); };
     const float top = value(first);
-    // exp(l - top); a logit of +inf counts as 1 and every finite one as 0 then
+    // exp(l - top); a logit of +inf counts as 1 and every finite one as 0 then. A
+    // sigmoid that is shared out among those of the chosen is exp(l - top) too where
+    // all are so small that 1 + exp(l) is 1: exp(l) itself keeps few bits below -87.
+    const bool shares = P.score == kMoeSoftmax || (P.normalize && top < -64.f);
     auto weight = [&](float v) {
-        if (P.score == kMoeSigmoid) return 1.f / (1.f + expf(-v));
-        return v == top ? 1.f : expf(v - top);
+        if (shares) return v == top ? 1.f : expf(v - top);
+        const float e = expf(-fabsf(v));
+        return (v < 0.f ? e : 1.f) / (1.f + e);
     };
     float w = mine >= 0 ? weight(value(mine_key)) : 0.f;
     if (P.normalize || P.score == kMoeSoftmax) {
@@ -95,7 +99,8 @@ __global__ void __launch_bounds__(32 * kRouteWarps) route_kernel(const MoeRoute 
         }
 #pragma unroll
         for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-        w = sum > 0.f ? w / sum : 0.f;
+        // (0 where the chosen sigmoids are, and so their sum)
+        w = sum > 0.f && (P.score == kMoeSoftmax || expf(top) > 0.f) ? w / sum : 0.f;
     }
     if (lane < P.k) {
         P.ids[t * P.k + lane] = mine;
