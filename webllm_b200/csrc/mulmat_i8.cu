@@ -140,20 +140,27 @@ __device__ __forceinline__ void tma_3d(uint32_t dst, const CUtensorMap* tm, int 
         "l"(tm), "r"(x), "r"(y), "r"(z), "r"(smem_u32(bar)), "l"(policy)
         : "memory");
 }
-// The same into this CTA's memory, signalled on the barrier of the pair's first CTA.
-__device__ __forceinline__ void tma_2d_pair(uint32_t dst, const CUtensorMap* tm, int x, int y, uint64_t* bar) {
+// The address, for all CTAs of the cluster, of what lies at p's place in CTA `rank`.
+__device__ __forceinline__ uint32_t in_cta(const void* p, uint32_t rank) {
+    uint32_t a;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(smem_u32(p)), "r"(rank));
+    return a;
+}
+// The same copies into this CTA's memory, signalled on the barrier of the pair's
+// first CTA (bar: an address of in_cta).
+__device__ __forceinline__ void tma_2d_pair(uint32_t dst, const CUtensorMap* tm, int x, int y, uint32_t bar) {
     asm volatile(
         "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(
             dst),
-        "l"(tm), "r"(x), "r"(y), "r"(smem_u32(bar) & 0xFEFFFFFFu)
+        "l"(tm), "r"(x), "r"(y), "r"(bar)
         : "memory");
 }
-__device__ __forceinline__ void tma_3d_pair(uint32_t dst, const CUtensorMap* tm, int x, int y, int z, uint64_t* bar,
+__device__ __forceinline__ void tma_3d_pair(uint32_t dst, const CUtensorMap* tm, int x, int y, int z, uint32_t bar,
                                             uint64_t policy) {
     asm volatile(
         "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes.L2::cache_hint [%0], [%1, {%2, %3, "
         "%4}], [%5], %6;" ::"r"(dst),
-        "l"(tm), "r"(x), "r"(y), "r"(z), "r"(smem_u32(bar) & 0xFEFFFFFFu), "l"(policy)
+        "l"(tm), "r"(x), "r"(y), "r"(z), "r"(bar), "l"(policy)
         : "memory");
 }
 // 16 bytes to shared memory: `bytes` of src, then zeros.
@@ -166,9 +173,7 @@ __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, uint32
 // cluster scope the arrive waits for the thread's global stores: 1500 clocks a
 // chunk, 144 us against 64 for 512 tokens in 8 of 64 experts, 2048 -> 2048.)
 __device__ __forceinline__ void mbar_arrive_at(uint64_t* bar, uint32_t rank) {
-    uint32_t remote;
-    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(smem_u32(bar)), "r"(rank));
-    asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(remote) : "memory");
+    asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(in_cta(bar, rank)) : "memory");
 }
 __device__ __forceinline__ void fence_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 // UMMA shared-memory descriptor: K-major, 128-byte swizzle, 8-row groups 1024
@@ -248,10 +253,8 @@ __device__ __forceinline__ void cluster_sync() {
 __device__ __forceinline__ void cluster_meet() {
     asm volatile("barrier.cluster.arrive.relaxed.aligned;\n\tbarrier.cluster.wait.aligned;" ::: "memory");
 }
-__device__ __forceinline__ void st_cluster(uint32_t local, uint32_t rank, int v) {
-    uint32_t remote;
-    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(local), "r"(rank));
-    asm volatile("st.shared::cluster.s32 [%0], %1;" ::"r"(remote), "r"(v) : "memory");
+__device__ __forceinline__ void st_cluster(const int* p, uint32_t rank, int v) {
+    asm volatile("st.shared::cluster.s32 [%0], %1;" ::"r"(in_cta(p, rank)), "r"(v) : "memory");
 }
 __device__ __forceinline__ int4 ld_cluster4(uint32_t local, uint32_t rank) {
     uint32_t remote;
@@ -512,6 +515,7 @@ __global__ void __launch_bounds__(GROUPED ? kThreads + 2 * kLoaders : kThreads, 
             Ring ring{stages};
             int filled = 0;  // stages filled so far, up to the ring's size
             const uint64_t policy = evict_first();
+            const uint32_t full0 = PAIR ? in_cta(full, 0) : 0;  // the pair's first CTA's
             bool ok = true;
             for (int i = item0; i < items && ok; i += item_step) {
                 const Item it = walk.at(i);
@@ -532,8 +536,8 @@ __global__ void __launch_bounds__(GROUPED ? kThreads + 2 * kLoaders : kThreads, 
                     for (int h = 0; h < kSub; ++h) {
                         const int k = (c * kSub + h) * kChunk;
                         if constexpr (PAIR) {
-                            tma_3d_pair(a + h * kABytes, &P.wmap, k, m0, it.e, &full[s], policy);
-                            if constexpr (!GROUPED) tma_2d_pair(b + h * b_bytes, &P.xmap, k, n0, &full[s]);
+                            tma_3d_pair(a + h * kABytes, &P.wmap, k, m0, it.e, full0 + 8 * s, policy);
+                            if constexpr (!GROUPED) tma_2d_pair(b + h * b_bytes, &P.xmap, k, n0, full0 + 8 * s);
                         } else {
                             tma_3d(a + h * kABytes, &P.wmap, k, m0, it.e, &full[s], policy);
                             if constexpr (!GROUPED) tma_2d(b + h * b_bytes, &P.xmap, k, n0, &full[s]);
@@ -744,7 +748,7 @@ __global__ void __launch_bounds__(GROUPED ? kThreads + 2 * kLoaders : kThreads, 
         // one item per cluster, so that the sum over the splits comes after all roles;
         // a tile that one CTA gave up on is summed by none
         if (*poisoned)
-            for (int r = 0; r < P.splits; ++r) st_cluster(smem_u32(&poison), r, 1);
+            for (int r = 0; r < P.splits; ++r) st_cluster(&poison, r, 1);
         __syncwarp();
         cluster_sync();
         if (item0 < items && !*poisoned) {
