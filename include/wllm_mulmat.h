@@ -311,7 +311,8 @@ int32_t wllm_dequantize(int32_t type, const void* src, float* dst, int64_t n, vo
  * device is, use no library workspace, allocate nothing and never wait, so
  * calls on several streams are independent and each may be captured into a
  * graph, its first one too. Inputs are not modified; an output may overlap no
- * input of its call (WLLM_STATUS_FAILED where the library can see it). Extents
+ * input of its call: WLLM_STATUS_FAILED where the range from its first to its last
+ * byte, what lies between its rows included, meets an input's. Extents
  * are not checked. K, M, N and n_tokens * n_used are at most 2^31 - 1024. A
  * device-side wait of the products that gave up (wllm_set_wait_limit) is told by
  * the first wllm_sync after the launch has ended; that waits for the library's
@@ -330,7 +331,9 @@ int32_t wllm_dequantize(int32_t type, const void* src, float* dst, int64_t n, vo
  * not both. Rows are tokens' activations, or, once, a weight's channels (from
  * wllm_dequantize, for example). Strides are in elements of x_type (F32, F16 or
  * BF16; up has x's), q_stride in bytes. Bytes of q behind a row's K values are
- * left as they are. */
+ * left as they are. Rows of x and up that do not start on 16-byte boundaries are
+ * read in whole aligned 16-byte words, so up to 15 bytes ahead of a row and behind
+ * it are read too (and dropped). */
 typedef struct wllm_quantize_i8_args {
     int32_t x_type;
     int32_t K, N;
@@ -420,7 +423,9 @@ int32_t wllm_mul_mat_id_i8(const wllm_mulmat_id_i8_args* args, void* stream);
 
 /* y[m + y_stride*t] = sum_j weights[t*n_used + j] * z[m + z_stride*(t*n_used + j)],
  * summed in f32 in the order of j and rounded once to y_type. z_type and y_type:
- * F32, F16 or BF16. */
+ * F32, F16 or BF16. A z in 16 bits takes half of the time of one in F32, but rounds
+ * each slot's row ahead of the sum, and F16 ends at 65504: a larger value of one
+ * slot is an infinity of the sum, however small its weight. */
 int32_t wllm_moe_combine(int32_t z_type, const void* z, int64_t z_stride, const float* weights, int32_t y_type, void* y,
                          int64_t y_stride, int32_t n_tokens, int32_t n_used, int32_t M, void* stream);
 

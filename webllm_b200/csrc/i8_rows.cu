@@ -18,15 +18,19 @@
 // every product of it is NaN.
 //
 // Bound: HBM (one read of the row, K + 4 bytes written): 8192 x 14336 bf16 in 54
-// us, 6.5 TB/s; 4096 x 14336 f32 in 43.5 us, 6.8 TB/s; silu(gate) * up of 32768
-// x 1536 bf16 in 55 us, 4.6 TB/s, there bound by its exponentials too. One CTA
-// per row; the
-// row's values stay in registers between the maximum and the rounding, so rows
+// us, 6.5 TB/s; 4096 x 14336 f32 in 43.5 us, 6.8 TB/s (above what HBM copies at:
+// part of it is still in L2). Behind a prologue not: silu(gate) * up of 32768 x
+// 1536 bf16 takes 57 us, 4.4 TB/s, with the SFU busy for 44 % of the time, an
+// instruction issued in 54 % and most waits for loads, of which 64 registers a
+// thread leave 32 warps an SM to have in flight; gelu(gate) * up of 8192 x 8192 bf16
+// 103 us, 3.3 TB/s (issue 69 %); RMS_NORM(x) * gain of 8192 x 4096 bf16 43 us, 2.3
+// TB/s (issue 42 %, waits for loads and for the gain, read value by value). One
+// CTA per row; the row's values stay in registers between the maximum and the rounding, so rows
 // up to 32 values a thread are read once; longer rows are read again (from L2)
 // in the second pass.
 // Threads: rows that are few take one 8-value vector a thread (latency), many
 // rows as many as its registers keep (fewer barriers a byte), and many short rows
-// a warp each, eight a CTA (25,960 x 256, silu(gate) * up: 14 us against 29
+// a warp each, eight a CTA (25,960 x 256, silu(gate) * up: 11 us against 29
 // with a CTA a row).
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>

@@ -32,9 +32,10 @@ __device__ __forceinline__ float to_f32(T v) {
 // bits in an unsigned order (0 for NaN and -inf, which are never chosen); each
 // of the k steps is one warp-wide maximum of the keys and one minimum of the
 // expert numbers that hold it, so ties go to the lowest expert. The weights
-// are computed once, lane j the j-th's. Bound: launch latency for few tokens,
-// the k dependent reductions for many (the logits are read once: 4 E bytes a
-// token): 8192 tokens, 8 of 128 experts, 8.6 us.
+// are computed once, lane j the j-th's. Bound: launch latency for few tokens, the
+// integer pipe for many (busy for 75 % of the time with the k walks over the keys;
+// the logits are read once: 4 E bytes a token): 8192 tokens, 8 of 128 experts, 7.9
+// us.
 constexpr int kRouteWarps = 4;
 
 template <typename T, int LANE>  // LANE: logits a lane holds, E <= 32 LANE
@@ -170,7 +171,8 @@ __global__ void __launch_bounds__(32 * kPlanWarps) plan_kernel(const int32_t* id
     }
     __syncthreads();
     // counts of a key: exclusive over the warps (a lane each), and the CTA's total
-    if (warps <= 4) {  // few warps: a thread for each key
+    if (warps <= 4) {
+        // few warps: a thread for each key
         for (int e = threadIdx.x; e < keys; e += blockDim.x) {
             int c[4], sum = 0;
 #pragma unroll
@@ -182,17 +184,18 @@ __global__ void __launch_bounds__(32 * kPlanWarps) plan_kernel(const int32_t* id
             }
             total[e] = sum;
         }
-    } else
-    for (int e = warp; e < keys; e += warps) {
-        const int c = lane < warps ? count[lane * keys + e] : 0;
-        int sum = c;
+    } else {
+        for (int e = warp; e < keys; e += warps) {
+            const int c = lane < warps ? count[lane * keys + e] : 0;
+            int sum = c;
 #pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const int u = __shfl_up_sync(0xffffffffu, sum, o);
-            if (lane >= o) sum += u;
+            for (int o = 1; o < 32; o <<= 1) {
+                const int u = __shfl_up_sync(0xffffffffu, sum, o);
+                if (lane >= o) sum += u;
+            }
+            if (lane < warps) count[lane * keys + e] = sum - c;
+            if (lane == 31) total[e] = sum;
         }
-        if (lane < warps) count[lane * keys + e] = sum - c;
-        if (lane == 31) total[e] = sum;
     }
     __syncthreads();
     if (ctas > 1) asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
@@ -265,7 +268,7 @@ __global__ void __launch_bounds__(32 * kPlanWarps) plan_kernel(const int32_t* id
 // y[t][m] = sum_j weight[t][j] z[t k + j][m], in f32 and in the order of j (no
 // atomics, so the sum does not depend on timing). Bound: HBM or L2, one read of
 // the slots' rows; a thread takes 16 bytes of each: 4096 tokens, 8 f16 rows of
-// 4096, 44 us, 6.9 TB/s.
+// 4096, 44 us, 6.9 TB/s (above what HBM copies at: part of it is still in L2).
 template <typename T, int N>
 __device__ __forceinline__ void load_n(const T* p, float (&v)[N]) {
     if constexpr (N == 1) {
